@@ -1,0 +1,269 @@
+// Block quantisation to e4m3 (fp8.cuh) and reading it back.
+//
+//   rows      x [M,K] -> data [M,K], scale [M,ceil(K/128)]: one scale for 128 values of a row
+//   permuted  the same rows written to the expert-major places of their tokens: x is read and quantised
+//             once and stored k times
+//   weight    w [G,N,K] -> data [G,N,K], scale [G,ceil(N/128),ceil(K/128)]: one scale for 128 x 128 values, so
+//             the same tensor serves the product with w and, read the other way, with its transpose
+//   read      data, scale -> bf16 rows (exact: an e4m3 number times a power of two)
+//
+// All four only move bytes; K is a multiple of 16, so that a thread holds 16
+// values (one 16-byte store) and eight lanes a block.
+#include "fp8.cuh"
+
+namespace moe {
+namespace {
+
+using namespace fp8;
+
+constexpr int kUnit = 16;  // values of one thread
+
+// 16 values of bf16 (two 16-byte loads) or fp32 (four).
+MOE_DEVICE void load_unit(const __nv_bfloat16* p, float (&v)[kUnit]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint4 q = __ldg(reinterpret_cast<const uint4*>(p) + h);
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[h * 8 + 2 * i] = bf16_lo(w[i]);
+      v[h * 8 + 2 * i + 1] = bf16_hi(w[i]);
+    }
+  }
+}
+MOE_DEVICE void load_unit(const float* p, float (&v)[kUnit]) {
+#pragma unroll
+  for (int h = 0; h < 4; ++h) {
+    const float4 q = __ldg(reinterpret_cast<const float4*>(p) + h);
+    v[4 * h] = q.x;
+    v[4 * h + 1] = q.y;
+    v[4 * h + 2] = q.z;
+    v[4 * h + 3] = q.w;
+  }
+}
+
+MOE_DEVICE float unit_amax(const float (&v)[kUnit]) {
+  float a = 0.f;
+#pragma unroll
+  for (int i = 0; i < kUnit; ++i) a = fmaxf(a, finite_abs(v[i]));
+  return a;
+}
+
+MOE_DEVICE uint4 unit_pack(const float (&v)[kUnit], float inv) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w[i] = pack4(scaled(v[4 * i], inv), scaled(v[4 * i + 1], inv), scaled(v[4 * i + 2], inv),
+                 scaled(v[4 * i + 3], inv));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+constexpr int kRowThreads8 = 128;
+constexpr int kMaxTopk = 32;
+
+// One CTA per row (grid-stride over rows). kPermute: the row goes to its
+// token's k destinations instead of its own place.
+template <typename T, bool kPermute>
+__global__ void __launch_bounds__(kRowThreads8) quantize_rows_kernel(
+    const T* __restrict__ x, int64_t rows, int units, int kb, const int64_t* __restrict__ map,
+    const int64_t* __restrict__ experts, int k, int64_t E, int64_t num_out,
+    uint4* __restrict__ data, uint8_t* __restrict__ scale) {
+  __shared__ int64_t s_dst[kMaxTopk];
+  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+    if (kPermute) {
+      __syncthreads();
+      if (threadIdx.x < k) {
+        const int64_t e = __ldg(experts + r * k + threadIdx.x);
+        int64_t d = -1;
+        if (e >= 0 && e < E) d = __ldg(map + r * E + e);
+        s_dst[threadIdx.x] = d < num_out ? d : -1;
+      }
+      __syncthreads();
+    }
+    for (int u0 = 0; u0 < units; u0 += kRowThreads8) {
+      const int u = u0 + threadIdx.x;
+      const bool in = u < units;
+      float v[kUnit] = {};
+      if (in) load_unit(x + (r * units + u) * kUnit, v);
+      float a = unit_amax(v);
+#pragma unroll
+      for (int off = 4; off > 0; off >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, off));
+      const uint32_t b = scale_byte(a);
+      const uint4 q = unit_pack(v, inverse_scale(b));
+      if (!in) continue;
+      if (kPermute) {
+        for (int j = 0; j < k; ++j) {
+          const int64_t d = s_dst[j];
+          if (d < 0) continue;
+          data[d * units + u] = q;
+          if ((u & 7) == 0) scale[d * kb + (u >> 3)] = static_cast<uint8_t>(b);
+        }
+      } else {
+        data[r * units + u] = q;
+        if ((u & 7) == 0) scale[r * kb + (u >> 3)] = static_cast<uint8_t>(b);
+      }
+    }
+  }
+}
+
+constexpr int kTileThreads = 256;
+
+// One CTA per 128 x 128 block of one weight matrix; a thread holds four units.
+template <typename T>
+__global__ void __launch_bounds__(kTileThreads) quantize_weight_kernel(
+    const T* __restrict__ w, int64_t N, int units, int kb, uint4* __restrict__ data,
+    uint8_t* __restrict__ scale) {
+  __shared__ float s_amax[kTileThreads / 32];
+  const int u = blockIdx.x * 8 + (threadIdx.x & 7);
+  const int64_t n0 = static_cast<int64_t>(blockIdx.y) * kBlock + (threadIdx.x >> 3);
+  const int64_t base = static_cast<int64_t>(blockIdx.z) * N;
+  float v[4][kUnit] = {};
+  float a = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t n = n0 + 32 * i;
+    if (u < units && n < N) load_unit(w + ((base + n) * units + u) * kUnit, v[i]);
+    a = fmaxf(a, unit_amax(v[i]));
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, off));
+  if (lane_id() == 0) s_amax[warp_id()] = a;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kTileThreads / 32; ++i) a = fmaxf(a, s_amax[i]);
+  const uint32_t b = scale_byte(a);
+  const float inv = inverse_scale(b);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t n = n0 + 32 * i;
+    if (u < units && n < N) data[(base + n) * units + u] = unit_pack(v[i], inv);
+  }
+  if (threadIdx.x == 0)
+    scale[(static_cast<int64_t>(blockIdx.z) * gridDim.y + blockIdx.y) * kb + blockIdx.x] =
+        static_cast<uint8_t>(b);
+}
+
+// 16 values per thread.
+__global__ void __launch_bounds__(256) dequantize_rows_kernel(const uint4* __restrict__ data,
+                                                              const uint8_t* __restrict__ scale,
+                                                              int64_t total, int units, int kb,
+                                                              uint4* __restrict__ out) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= total) return;
+  const int64_t r = i / units;
+  const int u = static_cast<int>(i - r * units);
+  const float s = scale_value(__ldg(scale + r * kb + (u >> 3)));
+  const uint4 q = __ldg(data + i);
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  uint32_t o[8];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 a = unpack2(w[j]), b = unpack2(w[j] >> 16);
+    o[2 * j] = pack_bf16x2(a.x * s, a.y * s);
+    o[2 * j + 1] = pack_bf16x2(b.x * s, b.y * s);
+  }
+  out[2 * i] = make_uint4(o[0], o[1], o[2], o[3]);
+  out[2 * i + 1] = make_uint4(o[4], o[5], o[6], o[7]);
+}
+
+bool aligned16(const void* a, const void* b) {
+  return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15) == 0;
+}
+
+template <bool kPermute, typename T>
+int launch_rows(const T* x, int64_t M, int64_t K, const int64_t* map, const int64_t* experts, int k,
+                int64_t E, int64_t num_out, void* data, void* scale, cudaStream_t s,
+                const char* who) {
+  const int64_t grid = M < (1 << 20) ? M : (1 << 20);
+  quantize_rows_kernel<T, kPermute><<<static_cast<unsigned>(grid), kRowThreads8, 0, s>>>(
+      x, M, static_cast<int>(K / kUnit), static_cast<int>((K + kBlock - 1) / kBlock), map, experts,
+      k, E, num_out, static_cast<uint4*>(data), static_cast<uint8_t*>(scale));
+  MOE_CUDA_CHECK_LAUNCH(who);
+  return MOE_OK;
+}
+
+}  // namespace
+}  // namespace moe
+
+using namespace moe;
+
+extern "C" int moe_quantize_fp8(const void* x, int32_t src_type, int64_t M, int64_t K, void* data,
+                                void* scale, moe_stream_t stream) {
+  MOE_REQUIRE(src_type == 0 || src_type == 1, "quantize_fp8: src_type must be 0 (bf16) or 1 (fp32)");
+  MOE_REQUIRE(M >= 0 && K >= 16 && K % 16 == 0 && K < (1ll << 31),
+              "quantize_fp8: M=%lld K=%lld (K must be a positive multiple of 16)", (long long)M,
+              (long long)K);
+  if (M == 0) return MOE_OK;
+  MOE_REQUIRE(x && data && scale, "quantize_fp8: null pointer");
+  MOE_REQUIRE(aligned16(x, data), "quantize_fp8: x and data must be 16-byte aligned");
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (src_type == 1)
+    return launch_rows<false>(static_cast<const float*>(x), M, K, nullptr, nullptr, 0, 0, 0, data,
+                              scale, s, "quantize_fp8 launch");
+  return launch_rows<false>(static_cast<const __nv_bfloat16*>(x), M, K, nullptr, nullptr, 0, 0, 0,
+                            data, scale, s, "quantize_fp8 launch");
+}
+
+extern "C" int moe_permute_fp8(const void* x, const int64_t* row_id_map_te,
+                               const int64_t* topk_experts, int32_t k, void* data, void* scale,
+                               int64_t T, int64_t H, int64_t E, int64_t num_out,
+                               moe_stream_t stream) {
+  MOE_REQUIRE(T >= 0 && E >= 1 && num_out >= 0, "permute_fp8: bad shape T=%lld E=%lld rows=%lld",
+              (long long)T, (long long)E, (long long)num_out);
+  MOE_REQUIRE(H >= 16 && H % 16 == 0 && H < (1ll << 31),
+              "permute_fp8: H=%lld must be a positive multiple of 16", (long long)H);
+  MOE_REQUIRE(k >= 1 && k <= kMaxTopk, "permute_fp8: k=%d out of [1,%d]", k, kMaxTopk);
+  if (T == 0 || num_out == 0) return MOE_OK;
+  MOE_REQUIRE(x && row_id_map_te && topk_experts && data && scale, "permute_fp8: null pointer");
+  MOE_REQUIRE(aligned16(x, data), "permute_fp8: x and data must be 16-byte aligned");
+  return launch_rows<true>(static_cast<const __nv_bfloat16*>(x), T, H, row_id_map_te, topk_experts,
+                           k, E, num_out, data, scale, reinterpret_cast<cudaStream_t>(stream),
+                           "permute_fp8 launch");
+}
+
+extern "C" int moe_quantize_fp8_weight(const void* w, int32_t src_type, int64_t G, int64_t N,
+                                       int64_t K, void* data, void* scale, moe_stream_t stream) {
+  MOE_REQUIRE(src_type == 0 || src_type == 1,
+              "quantize_fp8_weight: src_type must be 0 (bf16) or 1 (fp32)");
+  MOE_REQUIRE(G >= 0 && G <= 65535, "quantize_fp8_weight: G=%lld out of [0,65535]", (long long)G);
+  MOE_REQUIRE(N >= 1 && (N + kBlock - 1) / kBlock <= 65535, "quantize_fp8_weight: N=%lld out of range",
+              (long long)N);
+  MOE_REQUIRE(K >= 16 && K % 16 == 0 && K < (1ll << 31),
+              "quantize_fp8_weight: K=%lld must be a positive multiple of 16", (long long)K);
+  if (G == 0) return MOE_OK;
+  MOE_REQUIRE(w && data && scale, "quantize_fp8_weight: null pointer");
+  MOE_REQUIRE(aligned16(w, data), "quantize_fp8_weight: w and data must be 16-byte aligned");
+  const int units = static_cast<int>(K / kUnit);
+  const int kb = static_cast<int>((K + kBlock - 1) / kBlock);
+  const dim3 grid(kb, static_cast<unsigned>((N + kBlock - 1) / kBlock), static_cast<unsigned>(G));
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (src_type == 1)
+    quantize_weight_kernel<float><<<grid, kTileThreads, 0, s>>>(
+        static_cast<const float*>(w), N, units, kb, static_cast<uint4*>(data),
+        static_cast<uint8_t*>(scale));
+  else
+    quantize_weight_kernel<__nv_bfloat16><<<grid, kTileThreads, 0, s>>>(
+        static_cast<const __nv_bfloat16*>(w), N, units, kb, static_cast<uint4*>(data),
+        static_cast<uint8_t*>(scale));
+  MOE_CUDA_CHECK_LAUNCH("quantize_fp8_weight launch");
+  return MOE_OK;
+}
+
+extern "C" int moe_dequantize_fp8(const void* data, const void* scale, int64_t M, int64_t K,
+                                  void* out, moe_stream_t stream) {
+  MOE_REQUIRE(M >= 0 && K >= 16 && K % 16 == 0 && K < (1ll << 31),
+              "dequantize_fp8: M=%lld K=%lld (K must be a positive multiple of 16)", (long long)M,
+              (long long)K);
+  if (M == 0) return MOE_OK;
+  MOE_REQUIRE(data && scale && out, "dequantize_fp8: null pointer");
+  MOE_REQUIRE(aligned16(data, out), "dequantize_fp8: data and out must be 16-byte aligned");
+  const int units = static_cast<int>(K / kUnit);
+  const int64_t total = M * units;
+  MOE_REQUIRE((total + 255) / 256 <= 0x7fffffffll, "dequantize_fp8: M*K too large");
+  dequantize_rows_kernel<<<static_cast<unsigned>((total + 255) / 256), 256, 0,
+                           reinterpret_cast<cudaStream_t>(stream)>>>(
+      static_cast<const uint4*>(data), static_cast<const uint8_t*>(scale), total, units,
+      static_cast<int>((K + kBlock - 1) / kBlock), static_cast<uint4*>(out));
+  MOE_CUDA_CHECK_LAUNCH("dequantize_fp8 launch");
+  return MOE_OK;
+}

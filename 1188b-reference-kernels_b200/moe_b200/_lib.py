@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import threading
-from ctypes import c_char_p, c_int32, c_int64, c_size_t, c_void_p, POINTER
+from ctypes import c_char_p, c_float, c_int32, c_int64, c_size_t, c_void_p, POINTER
 
 from . import build as _build
 
@@ -104,6 +104,21 @@ _SIGNATURES = {
                               c_int32, c_void_p],
     "moe_ep_combine": [c_void_p, c_void_p, c_int32, c_int32, c_int64, c_void_p, c_void_p,
                        c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p],
+    "moe_router_group_topk": [c_void_p, c_void_p, c_int64, c_int64, c_int32, c_int32, c_int32,
+                              c_int32, c_int32, c_int32, c_float, c_void_p, c_void_p, c_void_p,
+                              c_void_p, c_void_p],
+    "moe_router_topk_backward": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                 c_int64, c_int64, c_int32, c_int32, c_int32, c_float, c_void_p,
+                                 c_void_p],
+    "moe_quantize_fp8": [c_void_p, c_int32, c_int64, c_int64, c_void_p, c_void_p, c_void_p],
+    "moe_quantize_fp8_weight": [c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_void_p,
+                                c_void_p],
+    "moe_dequantize_fp8": [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p],
+    "moe_permute_fp8": [c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_int64,
+                        c_int64, c_int64, c_int64, c_void_p],
+    "moe_grouped_gemm_fp8": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                             c_int64, c_int64, c_int64, c_int64, c_int64, c_int32, c_int32,
+                             c_void_p, c_size_t, c_void_p],
 }
 _RESTYPE = {"moe_b200_last_error": c_char_p}
 
@@ -126,7 +141,9 @@ _LAUNCHES = {"moe_topk_f32": 1, "moe_router_topk": 1, "moe_router_topk_placed": 
              "moe_grouped_gemm_plan_splits": 1, "moe_grouped_gemm_plan_ep": 1,
              "moe_grouped_gemm": 2, "moe_grouped_gemm_nn": 2, "moe_grouped_wgrad": 3,
              "moe_grouped_wgrad_dev": 3,
-             "moe_swiglu": 1}
+             "moe_swiglu": 1, "moe_router_group_topk": 1, "moe_router_topk_backward": 1,
+             "moe_quantize_fp8": 1, "moe_quantize_fp8_weight": 1, "moe_dequantize_fp8": 1,
+             "moe_permute_fp8": 1, "moe_grouped_gemm_fp8": 1}
 launch_count = 0
 
 _lock = threading.Lock()

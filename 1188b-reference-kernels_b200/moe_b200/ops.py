@@ -24,6 +24,7 @@ __all__ = [
     "permute_trans", "permute_device_error", "unpermute", "unpermute_weighted", "grouped_gemm", "GroupedGemmPlan",
     "grouped_wgrad", "grouped_wgrad_device_error", "swiglu", "router_logits", "router_gemm_topk", "router_gemm_fusable",
     "router_device_error", "permute_backward", "combine_backward", "swiglu_backward",
+    "router_group_topk", "router_topk_backward",
 ]
 
 
@@ -124,6 +125,112 @@ def router_topk(logits: torch.Tensor, k: int, score: str = "softmax", renorm: bo
                   1 if score == "softmax" else 0, 1 if renorm else 0, _p(tv), _p(ti), _p(rmap),
                   _p(probs), _stream(dev))
     return RouterOutput(tv, ti, rmap, probs)
+
+
+def router_group_topk(logits: torch.Tensor, k: int, score: str = "sigmoid", num_groups: int = 1,
+                      topk_groups: int = 1, group_score: str = "top2",
+                      bias: Optional[torch.Tensor] = None, renorm: bool = True, scale: float = 1.0,
+                      outputs: str = "all") -> RouterOutput:
+    """Router with a balance bias and expert groups.
+
+    s = sigmoid(logits) or softmax(logits) (score); c = s + bias, where the
+    bias [E] fp32 steers the selection and not the weights. The E experts are
+    num_groups equal contiguous groups, a group is worth the sum of its two
+    largest c (group_score="top2") or its largest ("max"); the topk_groups
+    best stay and the k experts with the largest c inside them are taken.
+    Weights are s of the taken experts, divided by their sum if renorm (0
+    where that sum is 0), times scale. Selection scores are formed and
+    compared in 64 bits, ties go to the lower group and expert.
+    outputs="all" or "maps" (skip topk_vals/topk_idx). k <= 16, E <= 1024,
+    num_groups <= 32.
+    """
+    _need_cuda("logits", logits)
+    _need_dtype("logits", logits, torch.float32)
+    if logits.dim() != 2:
+        raise ValueError("logits must be [T,E]")
+    if score not in ("sigmoid", "softmax"):
+        raise ValueError("score must be 'sigmoid' or 'softmax'")
+    if group_score not in ("top2", "max"):
+        raise ValueError("group_score must be 'top2' or 'max'")
+    if outputs not in ("all", "maps"):
+        raise ValueError("outputs must be 'all' or 'maps'")
+    lg = logits.contiguous()
+    t, e = lg.shape
+    if num_groups < 1 or e % num_groups:
+        raise ValueError(f"{e} experts do not form {num_groups} equal groups")
+    if not 1 <= topk_groups <= num_groups:
+        raise ValueError(f"topk_groups must be in [1,{num_groups}], got {topk_groups}")
+    if not 1 <= k <= e // num_groups * topk_groups:
+        raise ValueError(f"k={k} out of range for {topk_groups} groups of {e // num_groups} experts")
+    dev = lg.device
+    if bias is not None:
+        _need_cuda("bias", bias)
+        _need_dtype("bias", bias, torch.float32)
+        if bias.shape != (e,) or bias.device != dev:
+            raise ValueError(f"bias must be [{e}] on {dev}")
+        bias = bias.contiguous()
+    tv = ti = None
+    if outputs == "all":
+        tv = torch.empty((t, k), dtype=torch.float32, device=dev)
+        ti = torch.empty((t, k), dtype=torch.int64, device=dev)
+    rmap = torch.empty((t, e), dtype=torch.bool, device=dev)
+    probs = torch.empty((t, e), dtype=torch.float32, device=dev)
+    with torch.cuda.device(dev):
+        _lib.call("moe_router_group_topk", _p(lg), _p(bias), t, e, int(k),
+                  1 if score == "softmax" else 2, int(num_groups), int(topk_groups),
+                  1 if group_score == "top2" else 0, 1 if renorm else 0, float(scale), _p(tv),
+                  _p(ti), _p(rmap), _p(probs), _stream(dev))
+    return RouterOutput(tv, ti, rmap, probs)
+
+
+def router_topk_backward(logits: torch.Tensor, topk_idx: torch.Tensor,
+                         grad_vals: Optional[torch.Tensor] = None,
+                         grad_probs: Optional[torch.Tensor] = None, score: str = "softmax",
+                         renorm: bool = True, scale: float = 1.0,
+                         bias: Optional[torch.Tensor] = None,
+                         placement: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Gradient of the routing weights with respect to the logits, [T,E] fp32.
+
+    topk_idx [T,k]: the selection of router_topk or router_group_topk (k <= 32;
+    itself constant). The gradient of the weights comes as grad_vals [T,k] or
+    as grad_probs [T,E] (what MoELayer.backward returns; read at the selected
+    entries). score, renorm, scale: the router's ("logits", "softmax" or
+    "sigmoid"); bias: what router_topk added to the logits (None for
+    router_group_topk, whose bias steers the selection alone); placement: as
+    router_topk's (the result counts model experts).
+    """
+    for n_, t_ in (("logits", logits), ("topk_idx", topk_idx), ("grad_vals", grad_vals),
+                   ("grad_probs", grad_probs), ("bias", bias), ("placement", placement)):
+        _need_cuda(n_, t_)
+        if t_ is not None and t_.device != logits.device:
+            raise ValueError(f"{n_} is on {t_.device}, logits on {logits.device}")
+    _need_dtype("logits", logits, torch.float32)
+    _need_dtype("topk_idx", topk_idx, torch.int64)
+    modes = {"logits": 0, "softmax": 1, "sigmoid": 2}
+    if score not in modes:
+        raise ValueError("score must be 'logits', 'softmax' or 'sigmoid'")
+    if logits.dim() != 2 or topk_idx.dim() != 2 or topk_idx.shape[0] != logits.shape[0]:
+        raise ValueError(f"shapes logits {tuple(logits.shape)} topk_idx {tuple(topk_idx.shape)}")
+    t, e = logits.shape
+    k = topk_idx.shape[1]
+    if not 1 <= k <= min(e, 32):
+        raise ValueError(f"k={k} out of [1,{min(e, 32)}]")
+    if (grad_vals is None) == (grad_probs is None):
+        raise ValueError("pass exactly one of grad_vals [T,k] and grad_probs [T,E]")
+    for n_, t_, sh in (("grad_vals", grad_vals, (t, k)), ("grad_probs", grad_probs, (t, e)),
+                       ("bias", bias, (e,)), ("placement", placement, (e,))):
+        if t_ is not None:
+            _need_dtype(n_, t_, torch.int32 if n_ == "placement" else torch.float32)
+            if tuple(t_.shape) != sh:
+                raise ValueError(f"{n_} must be {sh}, got {tuple(t_.shape)}")
+    dev = logits.device
+    lg, ix, gv, gp, b, pl = (None if v is None else v.contiguous()
+                             for v in (logits, topk_idx, grad_vals, grad_probs, bias, placement))
+    out = torch.empty((t, e), dtype=torch.float32, device=dev)
+    with torch.cuda.device(dev):
+        _lib.call("moe_router_topk_backward", _p(lg), _p(b), _p(pl), _p(ix), _p(gv), _p(gp), t, e,
+                  k, modes[score], 1 if renorm else 0, float(scale), _p(out), _stream(dev))
+    return out
 
 
 # --------------------------------------------------------------------------- a3
@@ -327,12 +434,14 @@ class GroupedGemmPlan:
         self.workspace = _workspace(self.nbytes, device)
         self.workspace[:256].zero_()  # error word reads 0 before the first plan
         self.device = device
+        self.num_w = 0  # weight matrices that the table names, once it is built
 
     def from_splits(self, m_splits: torch.Tensor, align: int = 1) -> "GroupedGemmPlan":
         ms = m_splits.to(device=self.device, dtype=torch.int32).contiguous()
         if ms.numel() != self.num_groups:
             raise ValueError(f"m_splits has {ms.numel()} entries, plan has {self.num_groups}")
         self._keep = ms
+        self.num_w = self.num_groups
         _lib.call("moe_grouped_gemm_plan_splits", _p(ms), self.num_groups, int(align),
                   _p(self.workspace), self.nbytes, _stream(self.device))
         return self
@@ -342,6 +451,7 @@ class GroupedGemmPlan:
         if c.numel() != num_src * num_w or num_src * num_w != self.num_groups:
             raise ValueError("counts must be [num_src * num_w]")
         self._keep = c
+        self.num_w = int(num_w)
         _lib.call("moe_grouped_gemm_plan_ep", _p(c), int(num_src), int(num_w),
                   _p(self.workspace), self.nbytes, _stream(self.device))
         return self

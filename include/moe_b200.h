@@ -98,6 +98,44 @@ int moe_router_gemm_topk(const void* x, const void* w, const float* bias, int64_
                          float* topk_vals, int64_t* topk_idx, uint8_t* routing_map, float* probs,
                          int32_t* device_error, moe_stream_t stream);
 
+/* Router with a balance bias and expert groups (no reference counterpart):   */
+/*   s = softmax(logits) (score_mode 1) or sigmoid(logits) (score_mode 2);    */
+/*   c = s + bias (nullable [E] fp32; it steers the selection, not the        */
+/*   weights); the E experts are num_groups equal contiguous groups, a group  */
+/*   is worth its largest c (group_score 0) or the sum of its two largest     */
+/*   (1); the topk_groups best groups stay, and the k experts with the        */
+/*   largest c inside them are taken, in that order.                          */
+/*   weight = s of a taken expert, with renorm != 0 divided by their sum      */
+/*   (0 where that sum is 0), times scale.                                    */
+/* c and the group values are formed and compared in 64 bits; ties go to the  */
+/* lower group and the lower expert, a NaN ranks first. A softmax row whose   */
+/* logits are all -inf has scores 0. Outputs as moe_router_topk's.            */
+/* k <= 16, E <= 1024, num_groups <= 32, else MOE_ERR_UNSUPPORTED.            */
+int moe_router_group_topk(const float* logits, const float* bias, int64_t T, int64_t E, int32_t k,
+                          int32_t score_mode, int32_t num_groups, int32_t topk_groups,
+                          int32_t group_score, int32_t renorm, float scale, float* topk_vals,
+                          int64_t* topk_idx, uint8_t* routing_map, float* probs,
+                          moe_stream_t stream);
+
+/* Gradient of the routing weights with respect to the logits, for the        */
+/* selection topk_idx [T,k] of moe_router_topk / _placed / _group_topk (the   */
+/* selection itself is constant; no reference counterpart). s of mode 0       */
+/* (logits), 1 (softmax) or 2 (sigmoid) of logits + bias (nullable, the bias  */
+/* moe_router_topk adds before everything; null for _group_topk);             */
+/* ds_j = scale * g_j, with renorm scale * (g_j / S - sum_i g_i s_i / S^2),   */
+/* S = sum_i s_i; then dx_j = ds_j, s_j (1 - s_j) ds_j, or over the whole row */
+/* s_e (ds_e - sum_j ds_j s_j). Exactly one of grad_vals [T,k] and grad_probs */
+/* [T,E] (read at the selected entries alone) is given. placement: as in      */
+/* moe_router_topk_placed (topk_idx and grad_probs count slots; bias and      */
+/* grad_logits model experts). An index outside [0,E) is skipped; an expert   */
+/* named twice gets the sum of its gradients. grad_logits [T,E] fp32 is       */
+/* written whole. k <= 32.                                                    */
+int moe_router_topk_backward(const float* logits, const float* bias, const int32_t* placement,
+                             const int64_t* topk_idx, const float* grad_vals,
+                             const float* grad_probs, int64_t T, int64_t E, int32_t k,
+                             int32_t score_mode, int32_t renorm, float scale, float* grad_logits,
+                             moe_stream_t stream);
+
 /* ------------------------------------------------------------------------ */
 /* a3  routing_map [T,E] bool -> row_id_map, expert-major destinations:      */
 /*   row[t,e] = base[e] + #{t' <= t : map[t',e]} - 1 if map[t,e] else -1     */
@@ -297,6 +335,48 @@ int moe_grouped_gemm_check(const void* workspace, size_t workspace_bytes, moe_st
 
 /* a11 standalone: h[M,F] = bf16(silu(y[:, :F]) * y[:, F:]) for y [M,2F].    */
 int moe_swiglu(const void* y, void* h, int64_t M, int64_t F, moe_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
+/* 8-bit experts (no reference counterpart). A block of 128 values holds e4m3 */
+/* numbers and one power-of-two scale 2^e, kept as the byte e + 127 (E8M0): e */
+/* is the smallest integer with amax <= 448 * 2^e (at least -127; 0 for a     */
+/* block of zeros), so nothing saturates and a value meets one rounding.      */
+/* Infinities and NaN do not enter amax and become NaN. The last block of a   */
+/* row may be shorter. Data and scales are contiguous; K % 16 == 0; x, data   */
+/* and out 16-byte aligned. src_type: 0 bf16, 1 fp32.                         */
+/* moe_quantize_fp8: x [M,K] -> data [M,K], scale [M,ceil(K/128)].            */
+int moe_quantize_fp8(const void* x, int32_t src_type, int64_t M, int64_t K, void* data,
+                     void* scale, moe_stream_t stream);
+/* moe_quantize_fp8_weight: w [G,N,K] -> data [G,N,K] and one scale for a     */
+/* block of 128 x 128, [G,ceil(N/128),ceil(K/128)]. G <= 65535.               */
+int moe_quantize_fp8_weight(const void* w, int32_t src_type, int64_t G, int64_t N, int64_t K,
+                            void* data, void* scale, moe_stream_t stream);
+/* moe_dequantize_fp8: data [M,K], scale -> out [M,K] bf16 (exact).           */
+int moe_dequantize_fp8(const void* data, const void* scale, int64_t M, int64_t K, void* out,
+                       moe_stream_t stream);
+/* moe_permute_fp8: quantises the rows of x [T,H] bf16 and writes row t to    */
+/* data / scale rows map[t, topk_experts[t,j]], j < k (moe_permute_topk of    */
+/* the quantised rows, in one pass). Experts outside [0,E) and rows outside   */
+/* [0,num_out) are skipped; rows that nothing names stay untouched. k <= 32.  */
+int moe_permute_fp8(const void* x, const int64_t* row_id_map_te, const int64_t* topk_experts,
+                    int32_t k, void* data, void* scale, int64_t T, int64_t H, int64_t E,
+                    int64_t num_out, moe_stream_t stream);
+/* Grouped GEMM of such operands on the block-scaled tensor cores, fp32       */
+/* accumulation: out[r] = x[r] @ w[widx(g)]^T for the rows r of group g, with */
+/* x [x_rows,K], x_scale [x_rows,ceil(K/128)]; w_kn 0: w [num_w,N,K], w_scale */
+/* [num_w,ceil(N/128),ceil(K/128)]; w_kn 1: w [num_w,K,N], w_scale            */
+/* [num_w,ceil(K/128),ceil(N/128)], out[r] = x[r] @ w (the input gradient of  */
+/* the product above with the weight as it is; N % 16 == 0).                  */
+/* epilogue 0: out [x_rows,N] bf16, N % 8 == 0.                               */
+/* epilogue 1 (w_kn 0): N = 2F, F % 128 == 0, rows [0,F) of w gate, [F,2F)    */
+/*   up: silu(gate) * up quantised from fp32, out [x_rows,F] e4m3, out_scale  */
+/*   [x_rows,F/128]; pre (nullable) [x_rows,N] bf16 gets gate|up.             */
+/* Groups, workspace and device error word: as moe_grouped_gemm (plans of     */
+/* moe_grouped_gemm_plan_*). Rows in no group are left as they are.           */
+int moe_grouped_gemm_fp8(const void* x, const void* x_scale, const void* w, const void* w_scale,
+                         void* out, void* out_scale, void* pre, int64_t x_rows, int64_t G,
+                         int64_t num_w, int64_t N, int64_t K, int32_t w_kn, int32_t epilogue,
+                         const void* workspace, size_t workspace_bytes, moe_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
 /* Expert-parallel exchange over NVLink (e): receive buffers registered for  */
