@@ -17,6 +17,7 @@
 // Rows are described by the group table of moe_grouped_gemm_plan_*. Every
 // wait is bounded (2 s): on timeout the kernel records an error word, drains
 // its copies and MMAs, frees TMEM and returns.
+#include <algorithm>
 #include <mutex>
 
 #include "fp8.cuh"
@@ -27,6 +28,9 @@ namespace moe {
 namespace g8 {
 
 using fp8::kBlock;
+using gg::Tile;
+using gg::raise_abort;
+using gg::wait_drain;
 
 constexpr int BM = 128;
 constexpr int BN = 256;
@@ -34,11 +38,15 @@ constexpr int kStages = 4;
 constexpr int kThreads = 224;
 constexpr uint32_t kTileBytes = 128 * 128;             // 128 rows (or reduction rows) x 128 bytes
 constexpr uint32_t kStageBytes = 3 * kTileBytes;       // A, B columns 0..127, B columns 128..255
-constexpr int kSfStages = 2;
+constexpr int kSfStages = 6;                           // scale buffers in shared memory
+constexpr int kSfTmem = 2;                             // and in TMEM
+constexpr int kSfBatch = 4;                            // K groups whose scales are loaded at once
 constexpr uint32_t kSfBytes = 512 + 1024;              // 128 A rows and 256 B rows, one 32-bit cell each
-constexpr size_t kSmemBytes = 1024 + kStages * kStageBytes + kSfStages * kSfBytes + 256;
+constexpr size_t kSmemBytes = 1024 + kStages * kStageBytes + kSfStages * kSfBytes + 512;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kSfCol = 480;                       // TMEM columns of the scales: 4 for A, 8 for B per stage
+
+constexpr int64_t kSlabBytes = 32ll << 20;  // weight bytes walked per pass: they stay in L2 beside the rows
 
 constexpr int kErrProducer = 1;
 constexpr int kErrMma = 2;
@@ -63,8 +71,10 @@ struct Params {
   int num_kb;    // 128-blocks along K
   int n_blocks;  // 128-blocks along N
   int n_tiles;
+  int n_chunk;   // pair kernel: N-tiles walked per pass over a group's rows
   int b_mn;      // weight is [num_w, K, N]: B staged MN-major
   int epilogue;  // 0 bf16 out; 1 SwiGLU -> e4m3 rows
+  bool x_words, w_words;  // scale rows are whole 32-bit words
 };
 
 // Instruction descriptor, kind::mxf8f6f4: D fp32, A and B e4m3, E8M0 scales;
@@ -106,6 +116,10 @@ MOE_DEVICE void umma_mxf8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uin
       : "memory");
 }
 
+// The same in every lane, and known to be so by the compiler.
+MOE_DEVICE uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
+MOE_DEVICE bool all_lanes(bool v) { return __all_sync(0xffffffffu, v) != 0; }
+
 MOE_DEVICE void tma_load_3d(uint32_t dst, const void* tmap, int32_t x, int32_t y, int32_t z,
                             uint32_t bar) {
   asm volatile(
@@ -115,51 +129,10 @@ MOE_DEVICE void tma_load_3d(uint32_t dst, const void* tmap, int32_t x, int32_t y
       : "memory");
 }
 
-MOE_DEVICE bool wait_drain(uint32_t bar, uint32_t parity) {
-  const unsigned long long t0 = globaltimer_ns();
-  while (!mbar_try_wait(bar, parity))
-    if (globaltimer_ns() - t0 > kWaitTimeoutNs) return false;
-  return true;
-}
-
-MOE_DEVICE void raise_abort(volatile int* abort_flag, int32_t* err, int code) {
-  atomicCAS(err, 0, code);
-  *abort_flag = 1;
-  __threadfence_block();
-}
-
-// Tile t of the launch: group, then N-tile by N-tile with the group's M-tiles
-// innermost (they share the weight tile). Indices only grow, so the walk only
-// moves forward.
-struct Tile {
-  int g, m, n;
-};
-struct Walker {
-  const int32_t* rows;
-  int G, n_tiles;
-  int g = 0, mt = -1;
-  long long base = 0;
-  __device__ bool locate(long long t, Tile& tile) {
-    while (g < G) {
-      if (mt < 0) mt = (max(rows[g], 0) + BM - 1) / BM;
-      const long long cnt = static_cast<long long>(mt) * n_tiles;
-      if (t < base + cnt) break;
-      base += cnt;
-      ++g;
-      mt = -1;
-    }
-    if (g >= G) return false;
-    const int local = static_cast<int>(t - base);
-    tile.g = g;
-    tile.n = local / mt;
-    tile.m = local % mt;
-    return true;
-  }
-};
-
 // Four scale bytes kb0..kb0+3 of a row of `num_kb` bytes at p (1.0 past its
-// end), `step` bytes apart.
-MOE_DEVICE uint32_t scale_cell(const uint8_t* p, int64_t step, int kb0, int num_kb) {
+// end), `step` bytes apart; one load where every such row starts on a word.
+MOE_DEVICE uint32_t scale_cell(const uint8_t* p, int64_t step, int kb0, int num_kb, bool words) {
+  if (words) return __ldg(reinterpret_cast<const uint32_t*>(p + kb0));
   uint32_t w = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -167,6 +140,26 @@ MOE_DEVICE uint32_t scale_cell(const uint8_t* p, int64_t step, int kb0, int num_
     w |= b << (8 * i);
   }
   return w;
+}
+
+// This lane's scale cells of one 512-deep K group: rows row0 + lane + 32 c of
+// x, and weight row blocks nb0, nb1 (the same cell for all 128 of a block).
+MOE_DEVICE void load_scale_cells(const Params& p, int64_t row0, int64_t wi, int nb0, int nb1, int kg,
+                                 int lane, uint32_t (&a)[4], uint32_t (&b)[2]) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const int64_t r = row0 + c * 32 + lane;
+    a[c] = r < p.x_rows ? scale_cell(p.xs + r * p.num_kb, 1, kg * 4, p.num_kb, p.x_words) : 0x7F7F7F7Fu;
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int nb = h ? nb1 : nb0;
+    const int64_t w0 =
+        p.b_mn ? wi * p.num_kb * p.n_blocks + nb : (wi * p.n_blocks + nb) * p.num_kb;
+    b[h] = nb < p.n_blocks && wi < p.num_w
+               ? scale_cell(p.ws + w0, p.b_mn ? p.n_blocks : 1, kg * 4, p.num_kb, p.w_words)
+               : 0x7F7F7F7Fu;
+  }
 }
 
 __global__ void __launch_bounds__(kThreads, 1)
@@ -184,13 +177,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto empty_bar = [&](int s) { return bar0 + 8u * (kStages + s); };
   auto sf_full = [&](int s) { return bar0 + 8u * (2 * kStages + s); };
   auto sf_empty = [&](int s) { return bar0 + 8u * (2 * kStages + kSfStages + s); };
-  const uint32_t acc_full = bar0 + 8u * (2 * kStages + 2 * kSfStages);
+  auto sf_used = [&](int b) { return bar0 + 8u * (2 * kStages + 2 * kSfStages + b); };
+  const uint32_t acc_full = bar0 + 8u * (2 * kStages + 2 * kSfStages + kSfTmem);
   const uint32_t acc_empty = acc_full + 8u;
   const uint32_t drain_bar = acc_full + 16u;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 2 * kSfStages + 3);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 2 * kSfStages + kSfTmem + 3);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = warp_id();
+  const int warp = static_cast<int>(uniform(static_cast<uint32_t>(warp_id())));
   const int lane = lane_id();
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -201,6 +195,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(sf_full(s), 1);
       mbar_init(sf_empty(s), 1);
     }
+    for (int b = 0; b < kSfTmem; ++b) mbar_init(sf_used(b), 1);
     mbar_init(acc_full, 1);
     mbar_init(acc_empty, 4);
     mbar_init(drain_bar, 1);
@@ -218,10 +213,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = uniform(*tmem_slot);
   const int groups4 = (p.num_kb + 3) / 4;  // 512-deep K groups, one scale cell each
 
-  Walker walker{p.rows, p.G, p.n_tiles};
+  gg::WalkerRT<BM> walker{p.rows, p.G, p.n_tiles, 1 << 20, 0};
   Tile tile;
 
   if (warp == 0) {
@@ -234,9 +229,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int s = 0; s < kStages; ++s) issued[s] = -1;
       bool ok = true;
       for (long long t = blockIdx.x; ok && walker.locate(t, tile); t += gridDim.x) {
-        const int row0 = p.row_start[tile.g] + tile.m * BM;
+        const int row0 = p.row_start[tile.g] + tile.m_idx * BM;
         const int wi = p.widx[tile.g];
-        const int n0 = p.epilogue == 1 ? tile.n * 128 : tile.n * BN;
+        const int n0 = p.epilogue == 1 ? tile.n_idx * 128 : tile.n_idx * BN;
         const int n1 = p.epilogue == 1 ? p.f_half + n0 : n0 + 128;
         for (int kb = 0; kb < p.num_kb; ++kb) {
           if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag)) {
@@ -269,66 +264,99 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA issuer
-    if (lane == 0) {
+    // The whole warp runs the loop in step (every wait's answer is a vote) and
+    // one lane issues: the operands of an MMA are then warp-uniform registers.
+    // With the loop in one lane's branch an MMA took 240 clocks to issue,
+    // against the unit's own 128.
+    {
+      const bool issuer = lane == 0;
       const uint32_t idesc = idesc_mxf8(BM, BN, p.b_mn != 0);
       // +32 values along K: 32 bytes inside a K-major swizzle row; 32 reduction
       // rows (four 1024-byte groups of 8) of an MN-major tile.
       const uint64_t bstep = p.b_mn ? 4096ull >> 4 : 32ull >> 4;
-      int stage = 0, sf = 0;
+      int stage = 0, sf = 0, copied = 0, used = 0;
       uint32_t phase = 0, sf_phase = 0, acc_phase = 0;
-      bool ok = true, issued_any = false;
-      for (long long t = blockIdx.x; ok && walker.locate(t, tile); t += gridDim.x) {
-        if (!mbar_wait(acc_empty, acc_phase ^ 1u, abort_flag)) {
+      bool ok = true, issued_any = false, ready = false;
+      // Scales of the next K group (the CTA's groups in order, across tiles) to the
+      // TMEM buffer that the group before the current one has used. Called in
+      // the middle of a group, so that neither wait is for work just issued.
+      auto copy_scales = [&]() {
+        const uint32_t b = static_cast<uint32_t>(copied & 1);
+        if (!all_lanes(mbar_wait(sf_used(b), static_cast<uint32_t>((copied >> 1) & 1) ^ 1u, abort_flag) &&
+                       mbar_wait(sf_full(sf), sf_phase, abort_flag)))
+          return false;
+        tc_fence_after();
+        const uint32_t sfa = tmem + kSfCol + b * 12u;
+        const uint32_t src = sf_base + static_cast<uint32_t>(sf) * kSfBytes;
+        if (issuer) {
+          tmem_copy_scales(sfa, sf_desc(src));
+          tmem_copy_scales(sfa + 4u, sf_desc(src + 512u));
+          tmem_copy_scales(sfa + 8u, sf_desc(src + 1024u));
+          umma_commit(sf_empty(sf));
+        }
+        __syncwarp();
+        issued_any = true;
+        ++copied;
+        if (++sf == kSfStages) {
+          sf = 0;
+          sf_phase ^= 1u;
+        }
+        return true;
+      };
+      long long t = blockIdx.x;
+      bool more = all_lanes(walker.locate(t, tile));
+      if (more) ok = copy_scales();
+      while (ok && more) {
+        t += gridDim.x;
+        more = all_lanes(walker.locate(t, tile));  // whether another tile follows
+        if (!all_lanes(mbar_wait(acc_empty, acc_phase ^ 1u, abort_flag))) {
           ok = false;
           break;
         }
         tc_fence_after();
-        for (int kg = 0; kg < groups4 && ok; ++kg) {
-          if (!mbar_wait(sf_full(sf), sf_phase, abort_flag)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t sfa = tmem + kSfCol + static_cast<uint32_t>(sf) * 12u;
-          const uint32_t sfb = sfa + 4u;
-          const uint32_t src = sf_base + static_cast<uint32_t>(sf) * kSfBytes;
-          tmem_copy_scales(sfa, sf_desc(src));
-          tmem_copy_scales(sfb, sf_desc(src + 512u));
-          tmem_copy_scales(sfb + 4u, sf_desc(src + 1024u));
-          issued_any = true;
-          const int kb1 = min(kg * 4 + 4, p.num_kb);
-          for (int kb = kg * 4; kb < kb1; ++kb) {
-            if (!mbar_wait(full_bar(stage), phase, abort_flag)) {
+        for (int kg = 0; kg < groups4 && ok; ++kg, ++used) {
+          const uint32_t sfa = tmem + kSfCol + static_cast<uint32_t>(used & 1) * 12u;
+          const int n = min(4, p.num_kb - kg * 4);
+          for (int i = 0; i < n; ++i) {
+            if (!ready && !all_lanes(mbar_wait(full_bar(stage), phase, abort_flag))) {
               ok = false;
               break;
             }
+            // the next stage is looked at before this one's MMAs are issued,
+            // so that the answer's latency does not stand between the two
+            const int next = stage + 1 == kStages ? 0 : stage + 1;
+            ready = all_lanes(mbar_try_wait(full_bar(next), next == 0 ? phase ^ 1u : phase));
             tc_fence_after();
             const uint32_t sa = base + stage * kStageBytes;
             const uint64_t ad = umma_desc_k_sw128(sa);
             const uint64_t bd = p.b_mn ? umma_desc_mn_sw128(sa + kTileBytes, kTileBytes)
                                        : umma_desc_k_sw128(sa + kTileBytes);
-            const uint32_t id = with_sf_id(idesc, static_cast<uint32_t>(kb & 3));
+            const uint32_t id = with_sf_id(idesc, static_cast<uint32_t>(i));
+            if (issuer) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              umma_mxf8(tmem, ad + 2ull * k, bd + bstep * k, id, sfa, sfb, (kb | k) != 0 ? 1u : 0u);
-            umma_commit(empty_bar(stage));
+              for (int k = 0; k < 4; ++k)
+                umma_mxf8(tmem, ad + 2ull * k, bd + bstep * k, id, sfa, sfa + 4u,
+                      (kg | i | k) != 0 ? 1u : 0u);
+              umma_commit(empty_bar(stage));
+            }
+            __syncwarp();
             if (++stage == kStages) {
               stage = 0;
               phase ^= 1u;
             }
+            if (i == min(1, n - 1) && (kg + 1 < groups4 || more) && !copy_scales()) {
+              ok = false;
+              break;
+            }
           }
           if (!ok) break;
-          umma_commit(sf_empty(sf));
-          if (++sf == kSfStages) {
-            sf = 0;
-            sf_phase ^= 1u;
-          }
+          if (issuer) umma_commit(sf_used(used & 1));
         }
         if (!ok) break;
-        umma_commit(acc_full);
+        if (issuer) umma_commit(acc_full);
         acc_phase ^= 1u;
       }
-      if (!ok) {
+      if (!ok && issuer) {
         raise_abort(abort_flag, p.err, kErrMma);
         if (issued_any) {
           umma_commit(drain_bar);
@@ -343,41 +371,33 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t sf_phase = 0;
     bool ok = true;
     for (long long t = blockIdx.x; ok && walker.locate(t, tile); t += gridDim.x) {
-      const int64_t row0 = static_cast<int64_t>(p.row_start[tile.g]) + tile.m * BM;
+      const int64_t row0 = static_cast<int64_t>(p.row_start[tile.g]) + tile.m_idx * BM;
       const int64_t wi = p.widx[tile.g];
-      const int nb0 = p.epilogue == 1 ? tile.n : tile.n * 2;
-      const int nb1 = p.epilogue == 1 ? p.f_half / 128 + tile.n : nb0 + 1;
-      for (int kg = 0; kg < groups4; ++kg) {
-        uint32_t a[4];
+      const int nb0 = p.epilogue == 1 ? tile.n_idx : tile.n_idx * 2;
+      const int nb1 = p.epilogue == 1 ? p.f_half / 128 + tile.n_idx : nb0 + 1;
+      for (int kg0 = 0; kg0 < groups4 && ok; kg0 += kSfBatch) {
+        uint32_t a[kSfBatch][4], b[kSfBatch][2];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int64_t r = row0 + c * 32 + lane;
-          a[c] = r < p.x_rows ? scale_cell(p.xs + r * p.num_kb, 1, kg * 4, p.num_kb) : 0x7F7F7F7Fu;
-        }
-        uint32_t b[2];
+        for (int j = 0; j < kSfBatch; ++j)
+          if (kg0 + j < groups4) load_scale_cells(p, row0, wi, nb0, nb1, kg0 + j, lane, a[j], b[j]);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int nb = h ? nb1 : nb0;
-          const int64_t w0 = p.b_mn ? wi * p.num_kb * p.n_blocks + nb
-                                    : (wi * p.n_blocks + nb) * p.num_kb;
-          b[h] = nb < p.n_blocks && wi < p.num_w
-                     ? scale_cell(p.ws + w0, p.b_mn ? p.n_blocks : 1, kg * 4, p.num_kb)
-                     : 0x7F7F7F7Fu;
-        }
-        if (!mbar_wait(sf_empty(sf), sf_phase ^ 1u, abort_flag)) {
-          ok = false;
-          break;
-        }
-        uint4* dst = reinterpret_cast<uint4*>(sf_ptr + sf * kSfBytes) + lane;
-        dst[0] = make_uint4(a[0], a[1], a[2], a[3]);
-        dst[32] = make_uint4(b[0], b[0], b[0], b[0]);
-        dst[64] = make_uint4(b[1], b[1], b[1], b[1]);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(sf_full(sf));
-        if (++sf == kSfStages) {
-          sf = 0;
-          sf_phase ^= 1u;
+        for (int j = 0; j < kSfBatch; ++j) {
+          if (kg0 + j >= groups4) break;
+          if (!mbar_wait(sf_empty(sf), sf_phase ^ 1u, abort_flag)) {
+            ok = false;
+            break;
+          }
+          uint4* dst = reinterpret_cast<uint4*>(sf_ptr + sf * kSfBytes) + lane;
+          dst[0] = make_uint4(a[j][0], a[j][1], a[j][2], a[j][3]);
+          dst[32] = make_uint4(b[j][0], b[j][0], b[j][0], b[j][0]);
+          dst[64] = make_uint4(b[j][1], b[j][1], b[j][1], b[j][1]);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(sf_full(sf));
+          if (++sf == kSfStages) {
+            sf = 0;
+            sf_phase ^= 1u;
+          }
         }
       }
     }
@@ -395,12 +415,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       acc_phase ^= 1u;
       tc_fence_after();
-      const int m_local = tile.m * BM + quad * 32 + lane;
+      const int m_local = tile.m_idx * BM + quad * 32 + lane;
       const int64_t row = static_cast<int64_t>(p.row_start[tile.g]) + m_local;
       const bool rvalid = m_local < p.rows[tile.g] && row < p.x_rows;
       const uint32_t tbase = tmem + (static_cast<uint32_t>(quad * 32) << 16);
       if (p.epilogue == 0) {
-        const int n0 = tile.n * BN;
+        const int n0 = tile.n_idx * BN;
         __nv_bfloat16* orow = static_cast<__nv_bfloat16*>(p.out) + row * p.n;
 #pragma unroll 1
         for (int c = 0; c < BN / 32; ++c) {
@@ -427,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // are one block of the quantised output
         float h[128];
         float amax = 0.f;
-        __nv_bfloat16* prow = p.pre == nullptr ? nullptr : p.pre + row * p.n + tile.n * 128;
+        __nv_bfloat16* prow = p.pre == nullptr ? nullptr : p.pre + row * p.n + tile.n_idx * 128;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t gr[32], ur[32];
@@ -464,7 +484,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t sb = fp8::scale_byte(amax);
           const float inv = fp8::inverse_scale(sb);
           uint4* orow = reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) + row * p.f_half +
-                                                 tile.n * 128);
+                                                 tile.n_idx * 128);
 #pragma unroll
           for (int v = 0; v < 8; ++v) {
             uint32_t o[4];
@@ -476,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             orow[v] = make_uint4(o[0], o[1], o[2], o[3]);
           }
-          p.out_scale[row * (p.f_half / 128) + tile.n] = static_cast<uint8_t>(sb);
+          p.out_scale[row * (p.f_half / 128) + tile.n_idx] = static_cast<uint8_t>(sb);
         }
       }
       tc_fence_before();
@@ -491,6 +511,517 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// CTA-pair kernel (tcgen05 cta_group::2, clusters of 2): groups of at least
+// 256 rows, 256 x 256 tiles. Each CTA stages its own 128 A rows and half of
+// the B tile (32 KB a 128-block, six stages); the leader issues M=256, N=256
+// MMAs that read both CTAs' shared memory and scales and fill both TMEMs.
+// Every CTA keeps the scales of its own rows and of all 256 columns.
+//
+// TMEM: two accumulators of 256 columns and two scale buffers of 12 need 536
+// of 512 columns, so accumulator 1 starts at column 224 and the two share the
+// 32 columns 224..255. The epilogue reads those first and hands them over on
+// a barrier of their own (`shared`), which the next tile's MMAs wait for; the
+// rest of a tile's epilogue overlaps the next tile's mainloop.
+// ---------------------------------------------------------------------------
+namespace pairk {
+constexpr int kTileM = 256;
+constexpr int kStages = 6;
+constexpr uint32_t kStageBytes = 2 * kTileBytes;
+constexpr uint32_t kAccCol1 = 224;
+constexpr uint32_t kEpiWarpBytes = 4096;  // per epilogue warp: two 32 x 64-byte boxes or one 32 x 128-byte box
+constexpr size_t kSmemBytes =
+    1024 + kStages * kStageBytes + 4 * kEpiWarpBytes + kSfStages * kSfBytes + 512;
+static_assert(kSmemBytes <= 232448, "shared memory per CTA");
+}  // namespace pairk
+
+MOE_DEVICE void tma_load_3d_pair(uint32_t dst, const void* tmap, int32_t x, int32_t y, int32_t z,
+                                 uint32_t bar_cluster) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(bar_cluster)
+      : "memory");
+}
+
+MOE_DEVICE void tmem_copy_scales_pair(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc)
+               : "memory");
+}
+
+MOE_DEVICE void umma_mxf8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                               uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], "
+      "[%5], p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+      : "memory");
+}
+
+MOE_DEVICE void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c),
+               "r"(d)
+               : "memory");
+}
+
+__global__ void __launch_bounds__(kThreads, 1)
+    grouped_gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a,
+                                 const __grid_constant__ CUtensorMap tmap_b,
+                                 const __grid_constant__ CUtensorMap tmap_out,
+                                 const __grid_constant__ CUtensorMap tmap_pre, const Params p) {
+  using namespace pairk;
+  constexpr int kS = pairk::kStages;
+  constexpr uint32_t kSB = pairk::kStageBytes;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t base = (raw_addr + 1023u) & ~1023u;
+  uint8_t* base_ptr = smem_raw + (base - raw_addr);
+  const uint32_t epi_base = base + kS * kSB;
+  const uint32_t sf_base = epi_base + 4 * kEpiWarpBytes;
+  uint8_t* sf_ptr = base_ptr + kS * kSB + 4 * kEpiWarpBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sf_ptr + kSfStages * kSfBytes);
+  const uint32_t bar0 = smem_u32(bars);
+  auto full_bar = [&](int s) { return bar0 + 8u * s; };
+  auto empty_bar = [&](int s) { return bar0 + 8u * (kS + s); };
+  auto sf_full = [&](int s) { return bar0 + 8u * (2 * kS + s); };
+  auto sf_empty = [&](int s) { return bar0 + 8u * (2 * kS + kSfStages + s); };
+  auto sf_used = [&](int b) { return bar0 + 8u * (2 * kS + 2 * kSfStages + b); };
+  auto acc_full = [&](int a) { return bar0 + 8u * (2 * kS + 2 * kSfStages + kSfTmem + a); };
+  auto acc_empty = [&](int a) { return bar0 + 8u * (2 * kS + 2 * kSfStages + kSfTmem + 2 + a); };
+  const uint32_t shared_bar = bar0 + 8u * (2 * kS + 2 * kSfStages + kSfTmem + 4);
+  const uint32_t drain_bar = shared_bar + 8u;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kS + 2 * kSfStages + kSfTmem + 6);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const long long cid = cluster_id_x();
+  const long long ncl = num_clusters_x();
+  const int warp = static_cast<int>(uniform(static_cast<uint32_t>(warp_id())));
+  const int lane = lane_id();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kS; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int s = 0; s < kSfStages; ++s) {
+      mbar_init(sf_full(s), 2);  // the scale warps of both CTAs
+      mbar_init(sf_empty(s), 1);
+    }
+    for (int b = 0; b < kSfTmem; ++b) mbar_init(sf_used(b), 1);
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(acc_full(a), 1);
+      mbar_init(acc_empty(a), 8);  // four epilogue warps in each CTA
+    }
+    mbar_init(shared_bar, 8);
+    mbar_init(drain_bar, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmap_a);
+    tma_prefetch_desc(&tmap_b);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(tmem_slot), kTmemCols);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // barriers of both CTAs initialised before any remote use
+  tc_fence_after();
+  const uint32_t tmem = uniform(*tmem_slot);
+  const int groups4 = (p.num_kb + 3) / 4;
+
+  gg::WalkerRT<kTileM> walker{p.rows, p.G, p.n_tiles, 1 << 20, p.n_chunk};
+  Tile tile;
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- producer
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int issued[kS];
+#pragma unroll
+      for (int s = 0; s < kS; ++s) issued[s] = -1;
+      bool ok = true;
+      for (long long t = cid; ok && walker.locate(t, tile); t += ncl) {
+        const int row0 = p.row_start[tile.g] + tile.m_idx * kTileM + static_cast<int>(rank) * 128;
+        const int wi = p.widx[tile.g];
+        const int n0 = p.epilogue == 1 ? tile.n_idx * 128 + static_cast<int>(rank) * p.f_half
+                                       : tile.n_idx * BN + static_cast<int>(rank) * 128;
+        for (int kb = 0; kb < p.num_kb; ++kb) {
+          if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag)) {
+            ok = false;
+            break;
+          }
+          const uint32_t sa = base + stage * kSB;
+          const uint32_t leader_full = map_to_rank(full_bar(stage), 0);
+          if (leader) mbar_arrive_expect_tx(full_bar(stage), 2 * kSB);
+          tma_load_3d_pair(sa, &tmap_a, kb * 128, row0, 0, leader_full);
+          if (p.b_mn)
+            tma_load_3d_pair(sa + kTileBytes, &tmap_b, n0, kb * 128, wi, leader_full);
+          else
+            tma_load_3d_pair(sa + kTileBytes, &tmap_b, kb * 128, n0, wi, leader_full);
+          issued[stage] = static_cast<int>(phase);
+          if (++stage == kS) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      if (ok) {
+        // every stage's release lands in this CTA's shared memory: wait for the last ones
+        for (int s = 0; s < kS; ++s)
+          if (issued[s] >= 0) wait_drain(empty_bar(s), static_cast<uint32_t>(issued[s]));
+      } else {
+        raise_abort(abort_flag, p.err, kErrProducer);
+        if (leader) {
+          for (int s = 0; s < kS; ++s)
+            if (issued[s] >= 0) wait_drain(full_bar(s), static_cast<uint32_t>(issued[s]));
+        } else {
+          // copies count on the leader's barrier; give them a bounded time to land
+          const unsigned long long t0 = globaltimer_ns();
+          while (globaltimer_ns() - t0 < 200000ull) {
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA issuer (leader)
+    // The whole warp runs the loop in step (every wait's answer is a vote) and
+    // one lane issues: the operands of an MMA are then warp-uniform registers.
+    // With the loop in one lane's branch an MMA took 240 clocks to issue,
+    // against the unit's own 128.
+    if (leader) {
+      const bool issuer = lane == 0;
+      const uint32_t idesc = idesc_mxf8(kTileM, BN, p.b_mn != 0);
+      const uint64_t bstep = p.b_mn ? 4096ull >> 4 : 32ull >> 4;  // see grouped_gemm_fp8_kernel
+      int stage = 0, sf = 0, copied = 0, used = 0, it = 0;
+      uint32_t phase = 0, sf_phase = 0;
+      bool ok = true, issued_any = false, ready = false;
+      // Scales of the next K group (the pair's groups in order, across tiles) to the
+      // TMEM buffer that the group before the current one has used. Called in
+      // the middle of a group, so that neither wait is for work just issued.
+      auto copy_scales = [&]() {
+        const uint32_t b = static_cast<uint32_t>(copied & 1);
+        if (!all_lanes(mbar_wait(sf_used(b), static_cast<uint32_t>((copied >> 1) & 1) ^ 1u, abort_flag) &&
+                       mbar_wait_cluster(sf_full(sf), sf_phase, abort_flag)))
+          return false;
+        tc_fence_after();
+        const uint32_t sfa = tmem + kSfCol + b * 12u;
+        const uint32_t src = sf_base + static_cast<uint32_t>(sf) * kSfBytes;
+        if (issuer) {
+          tmem_copy_scales_pair(sfa, sf_desc(src));
+          tmem_copy_scales_pair(sfa + 4u, sf_desc(src + 512u));
+          tmem_copy_scales_pair(sfa + 8u, sf_desc(src + 1024u));
+          umma_commit_pair(sf_empty(sf), 0x3);
+        }
+        __syncwarp();
+        issued_any = true;
+        ++copied;
+        if (++sf == kSfStages) {
+          sf = 0;
+          sf_phase ^= 1u;
+        }
+        return true;
+      };
+      long long t = cid;
+      bool more = all_lanes(walker.locate(t, tile));
+      if (more) ok = copy_scales();
+      while (ok && more) {
+        t += ncl;
+        more = all_lanes(walker.locate(t, tile));  // whether another tile follows
+        const int acc = it & 1;
+        const uint32_t d_tmem = tmem + (acc ? kAccCol1 : 0u);
+        // the accumulator's last epilogue (two tiles ago) and the columns
+        // shared with the other accumulator's (the last tile)
+        if (!all_lanes(
+                mbar_wait_cluster(acc_empty(acc), static_cast<uint32_t>((it >> 1) & 1) ^ 1u, abort_flag) &&
+                mbar_wait_cluster(shared_bar, static_cast<uint32_t>(it & 1) ^ 1u, abort_flag))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        for (int kg = 0; kg < groups4 && ok; ++kg, ++used) {
+          const uint32_t sfa = tmem + kSfCol + static_cast<uint32_t>(used & 1) * 12u;
+          const int n = min(4, p.num_kb - kg * 4);
+          for (int i = 0; i < n; ++i) {
+            if (!ready && !all_lanes(mbar_wait(full_bar(stage), phase, abort_flag))) {
+              ok = false;
+              break;
+            }
+            // the next stage is looked at before this one's MMAs are issued,
+            // so that the answer's latency does not stand between the two
+            const int next = stage + 1 == kS ? 0 : stage + 1;
+            ready = all_lanes(mbar_try_wait(full_bar(next), next == 0 ? phase ^ 1u : phase));
+            tc_fence_after();
+            const uint32_t sa = base + stage * kSB;
+            const uint64_t ad = umma_desc_k_sw128(sa);
+            const uint64_t bd = p.b_mn ? umma_desc_mn_sw128(sa + kTileBytes, kTileBytes)
+                                       : umma_desc_k_sw128(sa + kTileBytes);
+            const uint32_t id = with_sf_id(idesc, static_cast<uint32_t>(i));
+            if (issuer) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                umma_mxf8_pair(d_tmem, ad + 2ull * k, bd + bstep * k, id, sfa, sfa + 4u,
+                      (kg | i | k) != 0 ? 1u : 0u);
+              umma_commit_pair(empty_bar(stage), 0x3);
+            }
+            __syncwarp();
+            if (++stage == kS) {
+              stage = 0;
+              phase ^= 1u;
+            }
+            if (i == min(1, n - 1) && (kg + 1 < groups4 || more) && !copy_scales()) {
+              ok = false;
+              break;
+            }
+          }
+          if (!ok) break;
+          if (issuer) umma_commit_pair(sf_used(used & 1), 0x1);
+        }
+        if (!ok) break;
+        if (issuer) umma_commit_pair(acc_full(acc), 0x3);
+        ++it;
+      }
+      if (!ok && issuer) {
+        raise_abort(abort_flag, p.err, kErrMma);
+        if (issued_any) {
+          umma_commit_pair(drain_bar, 0x1);
+          wait_drain(drain_bar, 0);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 6) {
+    // ---------------------------------------------------------------- scales
+    int sf = 0;
+    uint32_t sf_phase = 0;
+    int filled[kSfStages];
+#pragma unroll
+    for (int s = 0; s < kSfStages; ++s) filled[s] = -1;
+    bool ok = true;
+    for (long long t = cid; ok && walker.locate(t, tile); t += ncl) {
+      const int64_t row0 = static_cast<int64_t>(p.row_start[tile.g]) + tile.m_idx * kTileM + rank * 128;
+      const int64_t wi = p.widx[tile.g];
+      const int nb0 = p.epilogue == 1 ? tile.n_idx : tile.n_idx * 2;
+      const int nb1 = p.epilogue == 1 ? p.f_half / 128 + tile.n_idx : nb0 + 1;
+      for (int kg0 = 0; kg0 < groups4 && ok; kg0 += kSfBatch) {
+        uint32_t a[kSfBatch][4], b[kSfBatch][2];
+#pragma unroll
+        for (int j = 0; j < kSfBatch; ++j)
+          if (kg0 + j < groups4) load_scale_cells(p, row0, wi, nb0, nb1, kg0 + j, lane, a[j], b[j]);
+#pragma unroll
+        for (int j = 0; j < kSfBatch; ++j) {
+          if (kg0 + j >= groups4) break;
+          if (!mbar_wait_cluster(sf_empty(sf), sf_phase ^ 1u, abort_flag)) {
+            ok = false;
+            break;
+          }
+          uint4* dst = reinterpret_cast<uint4*>(sf_ptr + sf * kSfBytes) + lane;
+          dst[0] = make_uint4(a[j][0], a[j][1], a[j][2], a[j][3]);
+          dst[32] = make_uint4(b[j][0], b[j][0], b[j][0], b[j][0]);
+          dst[64] = make_uint4(b[j][1], b[j][1], b[j][1], b[j][1]);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(map_to_rank(sf_full(sf), 0));
+          filled[sf] = static_cast<int>(sf_phase);
+          if (++sf == kSfStages) {
+            sf = 0;
+            sf_phase ^= 1u;
+          }
+        }
+      }
+    }
+    if (!ok) {
+      if (lane == 0) raise_abort(abort_flag, p.err, kErrScales);
+    } else if (lane == 0) {
+      // the releases land in this CTA's shared memory: wait for the last ones
+      for (int s = 0; s < kSfStages; ++s)
+        if (filled[s] >= 0) wait_drain(sf_empty(s), static_cast<uint32_t>(filled[s]));
+    }
+    __syncwarp();
+  } else {
+    // ---------------------------------------------------------------- epilogue (both CTAs)
+    const int quad = warp & 3;
+    const uint32_t leader_empty0 = map_to_rank(acc_empty(0), 0);
+    const uint32_t leader_empty1 = map_to_rank(acc_empty(1), 0);
+    const uint32_t leader_shared = map_to_rank(shared_bar, 0);
+    const uint32_t epi = epi_base + static_cast<uint32_t>(quad) * kEpiWarpBytes;
+    uint32_t box_no = 0;
+    int it = 0;
+    bool ok = true;
+    for (long long t = cid; walker.locate(t, tile); t += ncl, ++it) {
+      const int acc = it & 1;
+      if (!mbar_wait_cluster(acc_full(acc), static_cast<uint32_t>((it >> 1) & 1), abort_flag)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const int m_local = tile.m_idx * kTileM + static_cast<int>(rank) * 128 + quad * 32 + lane;
+      const int64_t row = static_cast<int64_t>(p.row_start[tile.g]) + m_local;
+      const bool rvalid = m_local < p.rows[tile.g] && row < p.x_rows;
+      // a warp whose 32 rows all belong to the group stores them with TMA
+      const bool tma = __all_sync(0xffffffffu, rvalid);
+      const int warp_row0 = static_cast<int>(row) - lane;
+      const uint32_t tbase =
+          tmem + (static_cast<uint32_t>(quad * 32) << 16) + (acc ? kAccCol1 : 0u);
+      // 32 columns of bf16 of this lane's row through a 64-byte-swizzled box
+      auto emit = [&](const CUtensorMap* map, __nv_bfloat16* orow, const uint32_t (&o)[16], int col) {
+        if (tma) {
+          const uint32_t buf = epi + (box_no & 1u) * 2048u;
+          ++box_no;
+          if (lane == 0) bulk_wait_read<1>();  // the store that used this box has read it
+          __syncwarp();
+          const uint32_t sw = static_cast<uint32_t>((lane >> 1) & 3);
+#pragma unroll
+          for (uint32_t j = 0; j < 4; ++j)
+            st_shared_v4(buf + static_cast<uint32_t>(lane) * 64u + ((j ^ sw) << 4), o[4 * j],
+                         o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(map, col, warp_row0, buf);
+            bulk_commit();
+          }
+        } else if (rvalid) {
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            if (col + (v + 1) * 8 <= p.n)
+              *reinterpret_cast<uint4*>(orow + col + v * 8) =
+                  make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
+        }
+      };
+      auto release_shared = [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(leader_shared);
+      };
+      if (p.epilogue == 0) {
+        // accumulator 0 shares its last 32 columns, accumulator 1 its first
+        const int n0 = tile.n_idx * BN;
+        __nv_bfloat16* orow = static_cast<__nv_bfloat16*>(p.out) + row * p.n;
+#pragma unroll 1
+        for (int i = 0; i < 8; ++i) {
+          const int c = acc ? i : (i + 7) & 7;
+          uint32_t r[32];
+          tmem_ld_32x32b_x32(tbase + c * 32, r);
+          tmem_ld_wait();
+          if (i == 0) release_shared();
+          const int col = n0 + c * 32;
+          if (col >= p.n) continue;  // warp-uniform
+          uint32_t o[16];
+#pragma unroll
+          for (int q = 0; q < 16; ++q)
+            o[q] = pack_bf16x2(__uint_as_float(r[2 * q]), __uint_as_float(r[2 * q + 1]));
+          emit(&tmap_out, orow, o, col);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(acc ? leader_empty1 : leader_empty0);
+      } else {
+        // gate in columns 0..127, up in 128..255, 32 of each at a time; the
+        // shared columns lie in the chunk that comes first. h[] is indexed in
+        // the order of the chunks, so that it stays in registers.
+        float h[128];
+        float amax = 0.f;
+        __nv_bfloat16* prow = p.pre == nullptr ? nullptr : p.pre + row * p.n;
+        if (tma) {  // the last tile's box has been read before its bytes are used again
+          if (lane == 0) bulk_wait_read<0>();
+          __syncwarp();
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int c = acc ? i : (i + 3) & 3;
+          uint32_t gr[32], ur[32];
+          tmem_ld_32x32b_x32(tbase + c * 32, gr);
+          tmem_ld_32x32b_x32(tbase + 128 + c * 32, ur);
+          tmem_ld_wait();
+          if (i == 0) release_shared();
+          if (i == 3) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(acc ? leader_empty1 : leader_empty0);
+          }
+#pragma unroll
+          for (int q = 0; q < 16; ++q) {
+            const float2 v = swiglu2_f32(
+                make_float2(__uint_as_float(gr[2 * q]), __uint_as_float(gr[2 * q + 1])),
+                make_float2(__uint_as_float(ur[2 * q]), __uint_as_float(ur[2 * q + 1])));
+            h[i * 32 + 2 * q] = v.x;
+            h[i * 32 + 2 * q + 1] = v.y;
+            amax = fmaxf(amax, fmaxf(fp8::finite_abs(v.x), fp8::finite_abs(v.y)));
+          }
+          if (prow != nullptr) {
+            uint32_t o[16];
+#pragma unroll
+            for (int q = 0; q < 16; ++q)
+              o[q] = pack_bf16x2(__uint_as_float(gr[2 * q]), __uint_as_float(gr[2 * q + 1]));
+            emit(&tmap_pre, prow, o, tile.n_idx * 128 + c * 32);
+#pragma unroll
+            for (int q = 0; q < 16; ++q)
+              o[q] = pack_bf16x2(__uint_as_float(ur[2 * q]), __uint_as_float(ur[2 * q + 1]));
+            emit(&tmap_pre, prow, o, p.f_half + tile.n_idx * 128 + c * 32);
+          }
+        }
+        const uint32_t sb = fp8::scale_byte(amax);
+        const float inv = fp8::inverse_scale(sb);
+        if (tma) {
+          if (lane == 0) bulk_wait_read<0>();
+          __syncwarp();
+        }
+        uint8_t* orow = static_cast<uint8_t*>(p.out) + row * p.f_half + tile.n_idx * 128;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int c = acc ? i : (i + 3) & 3;
+#pragma unroll
+          for (int v = 0; v < 2; ++v) {
+            uint32_t o[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int j = i * 32 + v * 16 + q * 4;
+              o[q] = fp8::pack4(fp8::scaled(h[j], inv), fp8::scaled(h[j + 1], inv),
+                                fp8::scaled(h[j + 2], inv), fp8::scaled(h[j + 3], inv));
+            }
+            const uint32_t chunk = static_cast<uint32_t>(c * 2 + v);
+            if (tma)  // 128-byte-swizzled box of 32 rows
+              st_shared_v4(epi + static_cast<uint32_t>(lane) * 128u +
+                               ((chunk ^ static_cast<uint32_t>(lane & 7)) << 4),
+                           o[0], o[1], o[2], o[3]);
+            else if (rvalid)
+              *reinterpret_cast<uint4*>(orow + chunk * 16) = make_uint4(o[0], o[1], o[2], o[3]);
+          }
+        }
+        if (rvalid)
+          p.out_scale[row * (p.f_half / 128) + tile.n_idx] = static_cast<uint8_t>(sb);
+        if (tma) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&tmap_out, tile.n_idx * 128, warp_row0, epi);
+            bulk_commit();
+          }
+        }
+      }
+    }
+    if (lane == 0) bulk_wait_all();  // every tile store has finished
+    __syncwarp();
+    if (!ok && lane == 0) raise_abort(abort_flag, p.err, kErrEpilogue);
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // no CTA leaves while its partner may still touch its memory
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, kTmemCols);
   }
 }
 
@@ -517,16 +1048,64 @@ int make_tmap(CUtensorMap* m, const void* ptr, uint64_t d0, uint64_t d1, uint64_
   return MOE_OK;
 }
 
-int ensure_smem_attr(int dev) {
+// 2-D map over a row-major [rows, cols] output for 32-row tile stores: boxes
+// of 32 bf16 columns (64-byte swizzle) or 128 bytes (128-byte swizzle).
+int make_store_tmap(CUtensorMap* m, void* ptr, uint64_t cols, uint64_t rows, bool bf16) {
+  auto encode = gg::get_encode_fn();
+  cuuint64_t dims[2] = {cols, rows};
+  cuuint64_t strides[1] = {cols * (bf16 ? 2 : 1)};
+  cuuint32_t box[2] = {bf16 ? 32u : 128u, 32u};
+  cuuint32_t estr[2] = {1u, 1u};
+  const CUresult r = encode(
+      m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, ptr, dims,
+      strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+      bf16 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_last_error("grouped_gemm_fp8: cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+    return MOE_ERR_CUDA;
+  }
+  return MOE_OK;
+}
+
+// Launch attributes of both kernels, once per device; `clusters` gets the CTA
+// pairs that can be resident at once (0: none, the single-CTA kernel serves).
+int prepare_device(int dev, int* clusters) {
   static std::mutex mu;
+  static int pairs[64];
   static bool done[64] = {};
   std::lock_guard<std::mutex> lock(mu);
-  if (dev >= 0 && dev < 64 && done[dev]) return MOE_OK;
+  if (dev >= 0 && dev < 64 && done[dev]) {
+    *clusters = pairs[dev];
+    return MOE_OK;
+  }
   MOE_CUDA_CALL(cudaFuncSetAttribute(grouped_gemm_fp8_kernel,
                                      cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      static_cast<int>(kSmemBytes)),
                 "cudaFuncSetAttribute(grouped_gemm_fp8)");
-  if (dev >= 0 && dev < 64) done[dev] = true;
+  MOE_CUDA_CALL(cudaFuncSetAttribute(grouped_gemm_fp8_pair_kernel,
+                                     cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     static_cast<int>(pairk::kSmemBytes)),
+                "cudaFuncSetAttribute(grouped_gemm_fp8_pair)");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * 74);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = pairk::kSmemBytes;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, grouped_gemm_fp8_pair_kernel, &cfg) != cudaSuccess) n = 0;
+  cudaGetLastError();  // clear a non-sticky error of the query
+  if (dev >= 0 && dev < 64) {
+    pairs[dev] = n;
+    done[dev] = true;
+  }
+  *clusters = n;
   return MOE_OK;
 }
 
@@ -570,7 +1149,8 @@ extern "C" int moe_grouped_gemm_fp8(const void* x, const void* x_scale, const vo
               "grouped_gemm_fp8: x, w, out and pre must be 16-byte aligned");
   int dev = 0;
   MOE_CUDA_CALL(cudaGetDevice(&dev), "cudaGetDevice");
-  int st = g8::ensure_smem_attr(dev);
+  int clusters = 0;
+  int st = g8::prepare_device(dev, &clusters);
   if (st) return st;
 
   CUtensorMap ta, tb;
@@ -601,10 +1181,46 @@ extern "C" int moe_grouped_gemm_fp8(const void* x, const void* x_scale, const vo
   p.num_kb = static_cast<int>((K + 127) / 128);
   p.n_blocks = static_cast<int>((N + 127) / 128);
   p.n_tiles = epilogue == 1 ? p.f_half / 128 : static_cast<int>((N + g8::BN - 1) / g8::BN);
+  p.n_chunk = 0;
   p.b_mn = w_kn ? 1 : 0;
   p.epilogue = epilogue;
-  g8::grouped_gemm_fp8_kernel<<<num_sms(dev), g8::kThreads, g8::kSmemBytes,
-                                reinterpret_cast<cudaStream_t>(stream)>>>(ta, tb, p);
+  p.x_words = p.num_kb % 4 == 0 && (reinterpret_cast<uintptr_t>(x_scale) & 3) == 0;
+  p.w_words = !w_kn && p.num_kb % 4 == 0 && (reinterpret_cast<uintptr_t>(w_scale) & 3) == 0;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (clusters > 0) {
+    if (x_rows >= g8::pairk::kTileM) {  // fewer rows: no group has a whole pair tile
+      CUtensorMap to, tp;
+      st = g8::make_store_tmap(&to, out, static_cast<uint64_t>(epilogue == 1 ? p.f_half : p.n),
+                               static_cast<uint64_t>(x_rows), epilogue == 0);
+      if (st) return st;
+      tp = to;
+      if (pre != nullptr)
+        st = g8::make_store_tmap(&tp, pre, static_cast<uint64_t>(N), static_cast<uint64_t>(x_rows),
+                                 true);
+      if (st) return st;
+      g8::Params pb = p;
+      pb.rows = l.rows_body;
+      pb.n_chunk = static_cast<int>(
+          std::min<int64_t>(p.n_tiles, std::max<int64_t>(1, g8::kSlabBytes / (g8::BN * K))));
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(2 * clusters);
+      cfg.blockDim = dim3(g8::kThreads);
+      cfg.dynamicSmemBytes = g8::pairk::kSmemBytes;
+      cfg.stream = s;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = 2;
+      attr[0].val.clusterDim.y = 1;
+      attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      MOE_CUDA_CALL(cudaLaunchKernelEx(&cfg, g8::grouped_gemm_fp8_pair_kernel, ta, tb, to, tp, pb),
+                    "grouped_gemm_fp8 pair launch");
+    }
+    p.row_start = l.tail_start;
+    p.rows = l.rows_tail;
+  }
+  g8::grouped_gemm_fp8_kernel<<<num_sms(dev), g8::kThreads, g8::kSmemBytes, s>>>(ta, tb, p);
   MOE_CUDA_CHECK_LAUNCH("grouped_gemm_fp8 launch");
   return MOE_OK;
 }
