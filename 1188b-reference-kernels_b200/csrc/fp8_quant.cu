@@ -18,44 +18,94 @@ using namespace fp8;
 
 constexpr int kUnit = 16;  // values of one thread
 
-// 16 values of bf16 (two 16-byte loads) or fp32 (four).
-MOE_DEVICE void load_unit(const __nv_bfloat16* p, float (&v)[kUnit]) {
+// 16 values as they lie in memory. amax() is one instruction a value: the
+// largest magnitude, and not finite if any value is not; amax_finite() and
+// pack(.., true) then treat such a block as fp8.cuh says.
+struct Bf16Unit {
+  using T = __nv_bfloat16;
+  uint4 q[2];
+  MOE_DEVICE void load(const T* p) {
+    q[0] = __ldg(reinterpret_cast<const uint4*>(p));
+    q[1] = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+  }
+  MOE_DEVICE void zero() { q[0] = q[1] = make_uint4(0u, 0u, 0u, 0u); }
+  MOE_DEVICE uint32_t word(int i) const {
+    const uint4& v = q[i >> 2];
+    return (i & 3) == 0 ? v.x : (i & 3) == 1 ? v.y : (i & 3) == 2 ? v.z : v.w;
+  }
+  MOE_DEVICE float value(int i) const {
+    return (i & 1) ? bf16_hi(word(i >> 1)) : bf16_lo(word(i >> 1));
+  }
+  MOE_DEVICE float amax() const {
+    uint32_t a = word(0) & 0x7FFF7FFFu;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const uint4 q = __ldg(reinterpret_cast<const uint4*>(p) + h);
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    for (int i = 1; i < 8; ++i)
+      asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(a) : "r"(word(i) & 0x7FFF7FFFu));
+    return max_nan(bf16_lo(a), bf16_hi(a));
+  }
+  MOE_DEVICE static float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+  }
+};
+struct Fp32Unit {
+  using T = float;
+  float v[kUnit];
+  MOE_DEVICE void load(const T* p) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[h * 8 + 2 * i] = bf16_lo(w[i]);
-      v[h * 8 + 2 * i + 1] = bf16_hi(w[i]);
+    for (int h = 0; h < 4; ++h) {
+      const float4 q = __ldg(reinterpret_cast<const float4*>(p) + h);
+      v[4 * h] = q.x;
+      v[4 * h + 1] = q.y;
+      v[4 * h + 2] = q.z;
+      v[4 * h + 3] = q.w;
     }
   }
-}
-MOE_DEVICE void load_unit(const float* p, float (&v)[kUnit]) {
+  MOE_DEVICE void zero() {
 #pragma unroll
-  for (int h = 0; h < 4; ++h) {
-    const float4 q = __ldg(reinterpret_cast<const float4*>(p) + h);
-    v[4 * h] = q.x;
-    v[4 * h + 1] = q.y;
-    v[4 * h + 2] = q.z;
-    v[4 * h + 3] = q.w;
+    for (int i = 0; i < kUnit; ++i) v[i] = 0.f;
   }
-}
+  MOE_DEVICE float value(int i) const { return v[i]; }
+  MOE_DEVICE float amax() const {
+    float a = fabsf(v[0]);
+#pragma unroll
+    for (int i = 1; i < kUnit; ++i) a = Bf16Unit::max_nan(a, fabsf(v[i]));
+    return a;
+  }
+};
 
-MOE_DEVICE float unit_amax(const float (&v)[kUnit]) {
+template <typename U>
+MOE_DEVICE float amax_finite(const U& u) {
   float a = 0.f;
 #pragma unroll
-  for (int i = 0; i < kUnit; ++i) a = fmaxf(a, finite_abs(v[i]));
+  for (int i = 0; i < kUnit; ++i) a = fmaxf(a, finite_abs(u.value(i)));
   return a;
 }
 
-MOE_DEVICE uint4 unit_pack(const float (&v)[kUnit], float inv) {
+// `odd`: the block holds a value that is not finite.
+template <typename U>
+MOE_DEVICE uint4 pack(const U& u, float inv, bool odd) {
   uint32_t w[4];
+  if (!odd) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    w[i] = pack4(scaled(v[4 * i], inv), scaled(v[4 * i + 1], inv), scaled(v[4 * i + 2], inv),
-                 scaled(v[4 * i + 3], inv));
+    for (int i = 0; i < 4; ++i)
+      w[i] = pack4(u.value(4 * i) * inv, u.value(4 * i + 1) * inv, u.value(4 * i + 2) * inv,
+                   u.value(4 * i + 3) * inv);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = pack4(scaled(u.value(4 * i), inv), scaled(u.value(4 * i + 1), inv),
+                   scaled(u.value(4 * i + 2), inv), scaled(u.value(4 * i + 3), inv));
+  }
   return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+MOE_DEVICE float max8(float a) {  // over the eight lanes of a block
+#pragma unroll
+  for (int off = 4; off > 0; off >>= 1)
+    a = Bf16Unit::max_nan(a, __shfl_xor_sync(0xffffffffu, a, off));
+  return a;
 }
 
 constexpr int kRowThreads8 = 128;
@@ -63,9 +113,9 @@ constexpr int kMaxTopk = 32;
 
 // One CTA per row (grid-stride over rows). kPermute: the row goes to its
 // token's k destinations instead of its own place.
-template <typename T, bool kPermute>
+template <typename U, bool kPermute>
 __global__ void __launch_bounds__(kRowThreads8) quantize_rows_kernel(
-    const T* __restrict__ x, int64_t rows, int units, int kb, const int64_t* __restrict__ map,
+    const typename U::T* __restrict__ x, int64_t rows, int units, int kb, const int64_t* __restrict__ map,
     const int64_t* __restrict__ experts, int k, int64_t E, int64_t num_out,
     uint4* __restrict__ data, uint8_t* __restrict__ scale) {
   __shared__ int64_t s_dst[kMaxTopk];
@@ -83,13 +133,17 @@ __global__ void __launch_bounds__(kRowThreads8) quantize_rows_kernel(
     for (int u0 = 0; u0 < units; u0 += kRowThreads8) {
       const int u = u0 + threadIdx.x;
       const bool in = u < units;
-      float v[kUnit] = {};
-      if (in) load_unit(x + (r * units + u) * kUnit, v);
-      float a = unit_amax(v);
-#pragma unroll
-      for (int off = 4; off > 0; off >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, off));
+      U v;
+      v.zero();
+      if (in) v.load(x + (r * units + u) * kUnit);
+      float a = max8(v.amax());
+      const bool odd = !(a < INFINITY);
+      if (__any_sync(0xffffffffu, odd)) {
+        const float f = max8(amax_finite(v));
+        if (odd) a = f;
+      }
       const uint32_t b = scale_byte(a);
-      const uint4 q = unit_pack(v, inverse_scale(b));
+      const uint4 q = pack(v, inverse_scale(b), odd);
       if (!in) continue;
       if (kPermute) {
         for (int j = 0; j < k; ++j) {
@@ -106,37 +160,56 @@ __global__ void __launch_bounds__(kRowThreads8) quantize_rows_kernel(
   }
 }
 
-constexpr int kTileThreads = 256;
-
-// One CTA per 128 x 128 block of one weight matrix; a thread holds four units.
-template <typename T>
-__global__ void __launch_bounds__(kTileThreads) quantize_weight_kernel(
-    const T* __restrict__ w, int64_t N, int units, int kb, uint4* __restrict__ data,
+// One CTA per 128 x 128 block of one weight matrix; a thread holds kUnits
+// units (bf16: 4, 256 threads; fp32: 2, 512 threads: 32 registers of data
+// either way, so that enough blocks are resident to overlap one's loads with
+// another's stores).
+template <typename U, int kUnits>
+__global__ void __launch_bounds__(1024 / kUnits) quantize_weight_kernel(
+    const typename U::T* __restrict__ w, int64_t N, int units, int kb, uint4* __restrict__ data,
     uint8_t* __restrict__ scale) {
-  __shared__ float s_amax[kTileThreads / 32];
+  constexpr int kThreads = 1024 / kUnits, kRows = kThreads / 8;
+  __shared__ float s_amax[kThreads / 32];
   const int u = blockIdx.x * 8 + (threadIdx.x & 7);
   const int64_t n0 = static_cast<int64_t>(blockIdx.y) * kBlock + (threadIdx.x >> 3);
   const int64_t base = static_cast<int64_t>(blockIdx.z) * N;
-  float v[4][kUnit] = {};
+  U v[kUnits];
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    const int64_t n = n0 + kRows * i;
+    v[i].zero();
+    if (u < units && n < N) v[i].load(w + ((base + n) * units + u) * kUnit);
+  }
+  // the block's amax, of the finite values alone if there are others
+  auto block_max = [&](float a) {
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1)
+      a = Bf16Unit::max_nan(a, __shfl_xor_sync(0xffffffffu, a, off));
+    if (lane_id() == 0) s_amax[warp_id()] = a;
+    __syncthreads();
+    a = s_amax[0];
+#pragma unroll
+    for (int i = 1; i < kThreads / 32; ++i) a = Bf16Unit::max_nan(a, s_amax[i]);
+    return a;
+  };
   float a = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t n = n0 + 32 * i;
-    if (u < units && n < N) load_unit(w + ((base + n) * units + u) * kUnit, v[i]);
-    a = fmaxf(a, unit_amax(v[i]));
+  for (int i = 0; i < kUnits; ++i) a = Bf16Unit::max_nan(a, v[i].amax());
+  a = block_max(a);
+  const bool odd = !(a < INFINITY);
+  if (odd) {  // the whole block takes this branch
+    __syncthreads();
+    a = 0.f;
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) a = fmaxf(a, amax_finite(v[i]));
+    a = block_max(a);
   }
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, off));
-  if (lane_id() == 0) s_amax[warp_id()] = a;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kTileThreads / 32; ++i) a = fmaxf(a, s_amax[i]);
   const uint32_t b = scale_byte(a);
   const float inv = inverse_scale(b);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t n = n0 + 32 * i;
-    if (u < units && n < N) data[(base + n) * units + u] = unit_pack(v[i], inv);
+  for (int i = 0; i < kUnits; ++i) {
+    const int64_t n = n0 + kRows * i;
+    if (u < units && n < N) data[(base + n) * units + u] = pack(v[i], inv, odd);
   }
   if (threadIdx.x == 0)
     scale[(static_cast<int64_t>(blockIdx.z) * gridDim.y + blockIdx.y) * kb + blockIdx.x] =
@@ -170,13 +243,13 @@ bool aligned16(const void* a, const void* b) {
   return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15) == 0;
 }
 
-template <bool kPermute, typename T>
-int launch_rows(const T* x, int64_t M, int64_t K, const int64_t* map, const int64_t* experts, int k,
+template <bool kPermute, typename U>
+int launch_rows(const void* x, int64_t M, int64_t K, const int64_t* map, const int64_t* experts, int k,
                 int64_t E, int64_t num_out, void* data, void* scale, cudaStream_t s,
                 const char* who) {
   const int64_t grid = M < (1 << 20) ? M : (1 << 20);
-  quantize_rows_kernel<T, kPermute><<<static_cast<unsigned>(grid), kRowThreads8, 0, s>>>(
-      x, M, static_cast<int>(K / kUnit), static_cast<int>((K + kBlock - 1) / kBlock), map, experts,
+  quantize_rows_kernel<U, kPermute><<<static_cast<unsigned>(grid), kRowThreads8, 0, s>>>(
+      static_cast<const typename U::T*>(x), M, static_cast<int>(K / kUnit), static_cast<int>((K + kBlock - 1) / kBlock), map, experts,
       k, E, num_out, static_cast<uint4*>(data), static_cast<uint8_t*>(scale));
   MOE_CUDA_CHECK_LAUNCH(who);
   return MOE_OK;
@@ -198,9 +271,9 @@ extern "C" int moe_quantize_fp8(const void* x, int32_t src_type, int64_t M, int6
   MOE_REQUIRE(aligned16(x, data), "quantize_fp8: x and data must be 16-byte aligned");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (src_type == 1)
-    return launch_rows<false>(static_cast<const float*>(x), M, K, nullptr, nullptr, 0, 0, 0, data,
+    return launch_rows<false, Fp32Unit>(x, M, K, nullptr, nullptr, 0, 0, 0, data,
                               scale, s, "quantize_fp8 launch");
-  return launch_rows<false>(static_cast<const __nv_bfloat16*>(x), M, K, nullptr, nullptr, 0, 0, 0,
+  return launch_rows<false, Bf16Unit>(x, M, K, nullptr, nullptr, 0, 0, 0,
                             data, scale, s, "quantize_fp8 launch");
 }
 
@@ -216,7 +289,7 @@ extern "C" int moe_permute_fp8(const void* x, const int64_t* row_id_map_te,
   if (T == 0 || num_out == 0) return MOE_OK;
   MOE_REQUIRE(x && row_id_map_te && topk_experts && data && scale, "permute_fp8: null pointer");
   MOE_REQUIRE(aligned16(x, data), "permute_fp8: x and data must be 16-byte aligned");
-  return launch_rows<true>(static_cast<const __nv_bfloat16*>(x), T, H, row_id_map_te, topk_experts,
+  return launch_rows<true, Bf16Unit>(x, T, H, row_id_map_te, topk_experts,
                            k, E, num_out, data, scale, reinterpret_cast<cudaStream_t>(stream),
                            "permute_fp8 launch");
 }
@@ -238,11 +311,11 @@ extern "C" int moe_quantize_fp8_weight(const void* w, int32_t src_type, int64_t 
   const dim3 grid(kb, static_cast<unsigned>((N + kBlock - 1) / kBlock), static_cast<unsigned>(G));
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (src_type == 1)
-    quantize_weight_kernel<float><<<grid, kTileThreads, 0, s>>>(
+    quantize_weight_kernel<Fp32Unit, 2><<<grid, 512, 0, s>>>(
         static_cast<const float*>(w), N, units, kb, static_cast<uint4*>(data),
         static_cast<uint8_t*>(scale));
   else
-    quantize_weight_kernel<__nv_bfloat16><<<grid, kTileThreads, 0, s>>>(
+    quantize_weight_kernel<Bf16Unit, 4><<<grid, 256, 0, s>>>(
         static_cast<const __nv_bfloat16*>(w), N, units, kb, static_cast<uint4*>(data),
         static_cast<uint8_t*>(scale));
   MOE_CUDA_CHECK_LAUNCH("quantize_fp8_weight launch");

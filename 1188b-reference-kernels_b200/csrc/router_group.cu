@@ -8,8 +8,10 @@
 //   renorm, times scale. Ties go to the lower group and the lower expert.
 //
 // The selection hangs on the last bits of c wherever two experts come close
-// (16384 tokens x 256 experts always hold such pairs), so c and the group
-// values are formed and compared in 64 bits.
+// (16384 tokens x 256 experts always hold such pairs), so it is that of c and
+// group values formed and compared in 64 bits. A first pass in fp32 with an
+// error bound settles the rows where no decision is that close; the others
+// (one in some hundred) are selected in 64 bits.
 #include <math.h>
 
 #include "moe_common.cuh"
@@ -57,40 +59,38 @@ MOE_DEVICE float warp_maxf(float v) {
   return v;
 }
 
-// One warp per token, its c in shared memory as doubles.
-__global__ void __launch_bounds__(32 * kWarps) router_group_kernel(
-    const float* __restrict__ logits, const float* __restrict__ bias, int64_t T, int E, int k,
-    int softmax, int groups, int keep, int top2, int renorm, float scale, float* __restrict__ vals,
-    int64_t* __restrict__ idx_out, uint8_t* __restrict__ rmap, float* __restrict__ probs) {
-  extern __shared__ double s_c[];
-  const int lane = lane_id();
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * kWarps + warp_id();
-  if (t >= T) return;
-  double* c = s_c + warp_id() * E;
-  const float* x = logits + t * E;
-  double m = 0.0, z = 1.0;
-  if (softmax) {
-    float mf = -INFINITY;
-    for (int e = lane; e < E; e += 32) mf = fmaxf(mf, __ldg(x + e));
-    m = warp_maxf(mf);
-    double sum = 0.0;
-    for (int e = lane; e < E; e += 32) sum += exp(static_cast<double>(__ldg(x + e)) - m);
-    z = warp_sum(sum);
-  }
-  // A row without any score (every logit -inf) has softmax 0, not 0/0.
-  const bool none = softmax && m == -INFINITY;
-  auto score = [&](int e) -> double {
+// A token's logits as 64-bit scores.
+struct Scores64 {
+  const float* x;
+  const float* bias;
+  double m, z;
+  bool softmax, none;
+  // s of expert e; a softmax row whose every logit is -inf has s = 0
+  __device__ double s(int e) const {
     const double v = __ldg(x + e);
     if (!softmax) return 1.0 / (1.0 + exp(-v));
     return none ? (isnan(v) ? v : 0.0) : exp(v - m) / z;
-  };
-  for (int e = lane; e < E; e += 32) c[e] = score(e) + (bias ? static_cast<double>(__ldg(bias + e)) : 0.0);
+  }
+  __device__ double c(int e) const { return s(e) + (bias ? static_cast<double>(__ldg(bias + e)) : 0.0); }
+};
+
+// Softmax normaliser in 64 bits (all lanes).
+MOE_DEVICE double softmax_sum64(const float* x, int E, double m) {
+  double sum = 0.0;
+  for (int e = lane_id(); e < E; e += 32) sum += exp(static_cast<double>(__ldg(x + e)) - m);
+  return warp_sum(sum);
+}
+
+// Selection in 64 bits, the definition as it stands: returns lane r's (r < k)
+// expert. c: E doubles of this warp in shared memory.
+MOE_DEVICE int select64(const Scores64& sc, double* c, int E, int k, int groups, int keep, int top2) {
+  const int lane = lane_id();
+  for (int e = lane; e < E; e += 32) c[e] = sc.c(e);
   __syncwarp();
   const int size = E / groups;
   uint32_t kept = 0xffffffffu;  // bit g: group g stays
   if (keep < groups) {
     uint64_t key = 0;
-    int g = lane;
     if (lane < groups) {
       double a = -INFINITY, b = -INFINITY;  // the two largest; a NaN counts as the largest
       bool nan = false;
@@ -108,25 +108,21 @@ __global__ void __launch_bounds__(32 * kWarps) router_group_kernel(
     }
     kept = 0;
     for (int r = 0; r < keep; ++r) {
-      uint64_t w = key;
-      int wi = lane < groups ? g : 1 << 20;
-      if (kept >> lane & 1u) w = 0;
-      if (lane >= groups) w = 0;
       // a live key is never 0 (the smallest is that of -inf), so taken and
       // absent groups lose
+      uint64_t w = lane < groups && !(kept >> lane & 1u) ? key : 0;
+      int wi = lane < groups ? lane : 1 << 20;
       warp_argmax(w, wi);
       kept |= 1u << wi;
     }
   }
   int mine = 0;
-  double my_s = 0.0;
   uint32_t taken = 0;  // bit j: column lane + 32 j
   for (int r = 0; r < k; ++r) {
     uint64_t w = 0;
     int wi = 1 << 20;
     for (int e = lane, j = 0; e < E; e += 32, ++j) {
-      if (taken >> j & 1u) continue;
-      if (!(kept >> (e / size) & 1u)) continue;
+      if ((taken >> j & 1u) || !(kept >> (e / size) & 1u)) continue;
       const uint64_t key = order_key(c[e]);
       if (key > w) {
         w = key;
@@ -137,24 +133,214 @@ __global__ void __launch_bounds__(32 * kWarps) router_group_kernel(
     if ((wi & 31) == lane) taken |= 1u << (wi >> 5);
     if (lane == r) mine = wi;
   }
-  if (lane < k) my_s = score(mine);
-  double weight = my_s;
-  if (renorm) {
-    const double sum = warp_sum(my_s);
-    weight = sum == 0.0 ? 0.0 : my_s / sum;
+  return mine;
+}
+
+// Order-preserving bits of a float that is no NaN (-0 equal to +0); never 0.
+MOE_DEVICE uint32_t order_key32(float v) {
+  const uint32_t u = __float_as_uint(v + 0.0f);
+  return (u >> 31) ? ~u : (u | 0x80000000u);
+}
+MOE_DEVICE float key32_value(uint32_t key) {
+  return __uint_as_float((key >> 31) ? (key & 0x7fffffffu) : ~key);
+}
+
+struct RouteArgs {
+  const float* logits;
+  const float* bias;
+  int64_t T;
+  int E, k, softmax, groups, keep, top2, renorm;
+  float scale;
+  int lanes;  // lanes that share a group (a power of two)
+  int vpl;    // columns of a lane
+  float* vals;
+  int64_t* idx;
+  uint8_t* rmap;
+  float* probs;
+};
+
+// Fast selection in fp32 with an error bound. Each lane holds vpl consecutive
+// columns of one group, `lanes` lanes a group. c in fp32 is off by at most
+// `err` (below), so an order of fp32 values is the true one where neighbours
+// differ by more than 2 err. Returns false, in every lane, where a decision
+// hangs on less than that (0.5 % of the rows of normal logits), or at a NaN;
+// the caller then selects in 64 bits.
+template <int VPL>
+MOE_DEVICE bool select32(const RouteArgs& a, const float* x, int& mine) {
+  const int lane = lane_id();
+  const int size = a.E / a.groups;
+  const int g = lane / a.lanes;
+  const int first = (lane & (a.lanes - 1)) * a.vpl;  // inside the group
+  const int n = g < a.groups ? max(0, min(a.vpl, size - first)) : 0;
+  const int col0 = g * size + first;
+  float v[VPL], c[VPL];
+#pragma unroll
+  for (int j = 0; j < VPL; ++j) v[j] = j < n ? __ldg(x + col0 + j) : -INFINITY;
+  // fp32 scores and what they may be off by, in units of 2^-23.
+  // __expf(t) is off by 2 + 1.18 |t| of itself, __fdividef by 2.
+  // sigmoid: of exp's error s (1 - s) arrives, at most 1/4 * 2 + 1.18 * 0.23;
+  //   the sum 1 + e adds 1/2, the quotient 2: together below 4.
+  // softmax: t = x - m adds |t| / 2 to exp's; s |t| <= 1/e (z >= 1), so
+  //   s (2 + 1.68 |t|) <= 2 s + 0.62; z inherits the mean of 2 + 1.68 |t|
+  //   under s (at most 2 + 1.68 ln 512) and (16 + 5) / 2 for its own sums;
+  //   quotient and product add 2.5: together below 1 + 30 s, s <= 1 / z.
+  // Adding the bias rounds once more, 2^-24 |c|.
+  float m = 0.f, rz = 1.f, err;
+  if (a.softmax) {
+    m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) m = fmaxf(m, v[j]);
+    m = warp_maxf(m);
+    float z = 0.f;
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) z += j < n ? __expf(v[j] - m) : 0.f;
+    rz = __fdividef(1.0f, warp_sumf(z));
+    err = (1.f + 30.f * rz) * 1.1920929e-7f;
+  } else {
+    err = 4.f * 1.1920929e-7f;
   }
-  const float w = static_cast<float>(weight * static_cast<double>(scale));
-  if (lane < k) {
-    if (vals) vals[t * k + lane] = w;
-    if (idx_out) idx_out[t * k + lane] = mine;
+  bool odd = a.softmax && !(fabsf(m) < INFINITY);  // no maximum to subtract
+  float big = 0.f;
+#pragma unroll
+  for (int j = 0; j < VPL; ++j) {
+    c[j] = a.softmax ? __expf(v[j] - m) * rz : __fdividef(1.0f, 1.0f + __expf(-v[j]));
+    if (a.bias != nullptr && j < n) c[j] += __ldg(a.bias + col0 + j);
+    if (j < n) {
+      odd |= isnan(c[j]);
+      if (c[j] > -INFINITY) big = fmaxf(big, fabsf(c[j]));  // a bias of -inf is exact
+    }
   }
-  if (rmap)
-    for (int e = lane, j = 0; e < E; e += 32, ++j) rmap[t * E + e] = taken >> j & 1u;
-  if (probs) {
-    for (int e = lane; e < E; e += 32) probs[t * E + e] = 0.f;
-    __syncwarp();
-    if (lane < k) probs[t * E + mine] = w;
+  // __fdividef(1, y) is 0 for y in (2^126, inf), as sigmoid of such x is to
+  // within 2^-126
+  big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big)));
+  err += 5.9604645e-8f * big;
+  const float gap = 2.f * err;
+
+  bool in = n > 0;
+  if (a.keep < a.groups) {
+    float hi = -INFINITY, lo = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < VPL; ++j)
+      if (j < n) {
+        lo = fmaxf(lo, fminf(hi, c[j]));
+        hi = fmaxf(hi, c[j]);
+      }
+    for (int off = 1; off < a.lanes; off <<= 1) {
+      const float h2 = __shfl_xor_sync(0xffffffffu, hi, off);
+      const float l2 = __shfl_xor_sync(0xffffffffu, lo, off);
+      lo = fmaxf(fminf(hi, h2), fmaxf(lo, l2));
+      hi = fmaxf(hi, h2);
+    }
+    const float rank = a.top2 && size > 1 ? hi + lo : hi;
+    int better = 0;
+    for (int q = 0; q < a.groups; ++q)
+      better += __shfl_sync(0xffffffffu, rank, q * a.lanes) > rank;
+    const bool stays = g < a.groups && better < a.keep;
+    // worst group that stays against the best that goes: two sums of two
+    const uint32_t kept_min = __reduce_min_sync(0xffffffffu, stays ? order_key32(rank) : 0xffffffffu);
+    const uint32_t gone_max =
+        __reduce_max_sync(0xffffffffu, g < a.groups && !stays ? order_key32(rank) : 0u);
+    const int staying = __popc(__ballot_sync(0xffffffffu, stays && (lane & (a.lanes - 1)) == 0));
+    odd |= staying != a.keep || gone_max == 0u ||
+           !(key32_value(kept_min) - key32_value(gone_max) > 4.f * err + 4.f * 5.9604645e-8f * big);
+    in &= stays;
   }
+  uint32_t key[VPL];
+#pragma unroll
+  for (int j = 0; j < VPL; ++j) key[j] = in && j < n && !odd ? order_key32(c[j]) : 0u;
+  uint32_t best = 0;
+#pragma unroll
+  for (int j = 0; j < VPL; ++j) best = max(best, key[j]);
+  float last = INFINITY;
+  mine = 0;
+  for (int r = 0; r <= a.k; ++r) {  // one more than is taken: the border below
+    const uint32_t w = __reduce_max_sync(0xffffffffu, best);
+    if (w == 0u) {  // nothing left (all taken, or a NaN: odd)
+      odd |= r < a.k;
+      break;
+    }
+    const float value = key32_value(w);
+    odd |= !(last - value > gap);
+    last = value;
+    if (r == a.k) break;
+    const uint32_t owners = __ballot_sync(0xffffffffu, best == w);
+    const int owner = __ffs(owners) - 1;
+    odd |= (owners & (owners - 1)) != 0u;
+    int col = 0;
+    if (lane == owner) {
+      best = 0;
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) {
+        if (key[j] == w) {
+          key[j] = 0;
+          col = col0 + j;
+        }
+        best = max(best, key[j]);
+      }
+    }
+    col = __shfl_sync(0xffffffffu, col, owner);
+    if (lane == r) mine = col;
+  }
+  return !__any_sync(0xffffffffu, odd);
+}
+
+// One warp per token. VPL 0: 64 bits throughout (shapes whose lanes would
+// hold more than 16 columns).
+template <int VPL>
+__global__ void __launch_bounds__(32 * kWarps) router_group_kernel(const RouteArgs a) {
+  extern __shared__ double s_c[];
+  const int lane = lane_id();
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * kWarps + warp_id();
+  if (t >= a.T) return;
+  const float* x = a.logits + t * a.E;
+  // the dense outputs are 0 outside the selection
+  if (a.probs) {
+    float* row = a.probs + t * a.E;
+    if (a.E % 4 == 0 && (reinterpret_cast<uintptr_t>(a.probs) & 15) == 0)
+      for (int e = lane; e < a.E / 4; e += 32) reinterpret_cast<float4*>(row)[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+    else
+      for (int e = lane; e < a.E; e += 32) row[e] = 0.f;
+  }
+  if (a.rmap) {
+    uint8_t* row = a.rmap + t * a.E;
+    if (a.E % 4 == 0 && (reinterpret_cast<uintptr_t>(a.rmap) & 3) == 0)
+      for (int e = lane; e < a.E / 4; e += 32) reinterpret_cast<uint32_t*>(row)[e] = 0u;
+    else
+      for (int e = lane; e < a.E; e += 32) row[e] = 0;
+  }
+  int mine = 0;
+  bool done = false;
+  if constexpr (VPL > 0) done = select32<VPL>(a, x, mine);
+  Scores64 sc{x, a.bias, 0.0, 1.0, a.softmax != 0, false};
+  // The softmax's normaliser cancels in renormalised weights, so that only
+  // the 64-bit selection and plain softmax weights need it.
+  if (a.softmax) {
+    float m = -INFINITY;
+    for (int e = lane; e < a.E; e += 32) m = fmaxf(m, __ldg(x + e));
+    sc.m = warp_maxf(m);
+    sc.none = sc.m == -INFINITY;
+    if (!done || !a.renorm) sc.z = softmax_sum64(x, a.E, sc.m);
+  }
+  if (!done) mine = select64(sc, s_c + warp_id() * a.E, a.E, a.k, a.groups, a.keep, a.top2);
+  double weight = lane < a.k ? sc.s(mine) : 0.0;
+  if (a.renorm) {
+    const double sum = warp_sum(weight);
+    weight = sum == 0.0 ? 0.0 : weight / sum;
+  }
+  const float w = static_cast<float>(weight * static_cast<double>(a.scale));
+  __syncwarp();  // the zeros above come first
+  if (lane < a.k) {
+    if (a.vals) a.vals[t * a.k + lane] = w;
+    if (a.idx) a.idx[t * a.k + lane] = mine;
+    if (a.rmap) a.rmap[t * a.E + mine] = 1;
+    if (a.probs) a.probs[t * a.E + mine] = w;
+  }
+}
+
+template <int VPL>
+void launch_route(const RouteArgs& a, cudaStream_t s) {
+  router_group_kernel<VPL><<<static_cast<unsigned>((a.T + kWarps - 1) / kWarps), 32 * kWarps,
+                             kWarps * a.E * sizeof(double), s>>>(a);
 }
 
 // One warp per token; lane j < k holds the j-th selected expert.
@@ -225,7 +411,12 @@ __global__ void __launch_bounds__(32 * kWarps) router_backward_kernel(
     const float dj = __shfl_sync(0xffffffffu, ds, j);
     if (cj == col) dsum += dj;
   }
-  for (int e = lane; e < E; e += 32) o[e] = row_softmax ? -score(e) * dot : 0.f;
+  if (row_softmax)
+    for (int e = lane; e < E; e += 32) o[e] = -score(e) * dot;
+  else if (E % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0)
+    for (int e = lane; e < E / 4; e += 32) reinterpret_cast<float4*>(o)[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+  else
+    for (int e = lane; e < E; e += 32) o[e] = 0.f;
   __syncwarp();
   if (col >= 0) {
     float d = dsum;
@@ -269,10 +460,40 @@ extern "C" int moe_router_group_topk(const float* logits, const float* bias, int
   MOE_REQUIRE(topk_vals || topk_idx || routing_map || probs, "router_group_topk: no output requested");
   MOE_REQUIRE(logits != nullptr, "router_group_topk: null logits");
   MOE_REQUIRE(T <= (int64_t)0x7fffffff * kWarps, "router_group_topk: T too large");
-  router_group_kernel<<<static_cast<unsigned>((T + kWarps - 1) / kWarps), 32 * kWarps,
-                        kWarps * E * sizeof(double), reinterpret_cast<cudaStream_t>(stream)>>>(
-      logits, bias, T, static_cast<int>(E), k, score_mode == 1, num_groups, topk_groups,
-      group_score, renorm, scale, topk_vals, topk_idx, routing_map, probs);
+  RouteArgs a;
+  a.logits = logits;
+  a.bias = bias;
+  a.T = T;
+  a.E = static_cast<int>(E);
+  a.k = k;
+  a.softmax = score_mode == 1;
+  a.groups = num_groups;
+  a.keep = topk_groups;
+  a.top2 = group_score;
+  a.renorm = renorm;
+  a.scale = scale;
+  a.vals = topk_vals;
+  a.idx = topk_idx;
+  a.rmap = routing_map;
+  a.probs = probs;
+  a.lanes = 32;
+  while (32 / a.lanes < num_groups) a.lanes >>= 1;
+  a.vpl = (a.E / num_groups + a.lanes - 1) / a.lanes;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (a.vpl <= 1)
+    launch_route<1>(a, s);
+  else if (a.vpl <= 2)
+    launch_route<2>(a, s);
+  else if (a.vpl <= 4)
+    launch_route<4>(a, s);
+  else if (a.vpl <= 8)
+    launch_route<8>(a, s);
+  else if (a.vpl <= 12)
+    launch_route<12>(a, s);
+  else if (a.vpl <= 16)
+    launch_route<16>(a, s);
+  else
+    launch_route<0>(a, s);
   MOE_CUDA_CHECK_LAUNCH("router_group_topk launch");
   return MOE_OK;
 }

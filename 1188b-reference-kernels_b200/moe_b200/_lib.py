@@ -153,6 +153,8 @@ _lib = None
 def load(path=None, build_if_missing: bool = False):
     """Loads (once) and returns the ctypes handle of libmoe_b200.so."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib

@@ -14,7 +14,7 @@ from typing import NamedTuple, Optional, Sequence, Union
 import torch
 
 from . import _lib
-from .ops import GroupedGemmPlan, _need_cuda, _need_dtype, _p, _stream
+from .ops import GroupedGemmPlan, _need_cuda, _need_dtype, _on, _p, _stream
 
 __all__ = ["Fp8Tensor", "quantize_fp8", "quantize_fp8_weight", "dequantize_fp8", "permute_fp8",
            "grouped_gemm_fp8"]
@@ -83,7 +83,7 @@ def quantize_fp8(x: torch.Tensor) -> Fp8Tensor:
     _need_k("x", k)
     xc = _aligned(x)
     out = _empty((m, k), (m, _blocks(k)), dev)
-    with torch.cuda.device(dev):
+    with _on(dev):
         _lib.call("moe_quantize_fp8", _p(xc), src, m, k, _p(out.data), _p(out.scale), _stream(dev))
     return out
 
@@ -99,7 +99,7 @@ def quantize_fp8_weight(w: torch.Tensor) -> Fp8Tensor:
     _need_k("w", k)
     wc = _aligned(w)
     out = _empty((g, n, k), (g, _blocks(n), _blocks(k)), dev)
-    with torch.cuda.device(dev):
+    with _on(dev):
         _lib.call("moe_quantize_fp8_weight", _p(wc), src, g, n, k, _p(out.data), _p(out.scale),
                   _stream(dev))
     return out
@@ -115,7 +115,7 @@ def dequantize_fp8(q: Fp8Tensor) -> torch.Tensor:
     _need_k("q.data", k)
     data, scale = _aligned(q.data), q.scale.contiguous()
     out = torch.empty((m, k), dtype=torch.bfloat16, device=dev)
-    with torch.cuda.device(dev):
+    with _on(dev):
         _lib.call("moe_dequantize_fp8", _p(data), _p(scale), m, k, _p(out), _stream(dev))
     return out
 
@@ -143,7 +143,7 @@ def permute_fp8(x: torch.Tensor, row_id_map: torch.Tensor, experts: torch.Tensor
     _need_k("x", h)
     xc, mc, ec = _aligned(x), row_id_map.contiguous(), experts.contiguous()
     out = _empty((int(num_out), h), (int(num_out), _blocks(h)), dev)
-    with torch.cuda.device(dev):
+    with _on(dev):
         _lib.call("moe_permute_fp8", _p(xc), _p(mc), _p(ec), ec.shape[1], _p(out.data),
                   _p(out.scale), t, h, mc.shape[1], int(num_out), _stream(dev))
     return out
@@ -196,7 +196,7 @@ def grouped_gemm_fp8(x: Fp8Tensor, w: Fp8Tensor,
             if sum(int(v) for v in m_splits) > rows:
                 raise ValueError("sum(m_splits) exceeds x rows")
             m_splits = torch.tensor([int(v) for v in m_splits], dtype=torch.int32)
-        with torch.cuda.device(dev):
+        with _on(dev):
             plan = GroupedGemmPlan(g, dev).from_splits(m_splits)
     if plan.num_w != g or plan.workspace.device != dev:
         raise ValueError(f"plan names {plan.num_w} weight matrices on {plan.workspace.device}, w has "
@@ -209,7 +209,7 @@ def grouped_gemm_fp8(x: Fp8Tensor, w: Fp8Tensor,
         out, out_scale = _empty((rows, n // 2), (rows, n // 2 // BLOCK), dev)
         if return_pre:
             pre = torch.empty((rows, n), dtype=torch.bfloat16, device=dev)
-    with torch.cuda.device(dev):
+    with _on(dev):
         _lib.call("moe_grouped_gemm_fp8", _p(xd), _p(xs), _p(wd), _p(ws), _p(out), _p(out_scale),
                   _p(pre), rows, plan.num_groups, g, n, k, 1 if w_layout == "KN" else 0,
                   codes[epilogue], _p(plan.workspace), plan.nbytes, _stream(dev))

@@ -29,7 +29,27 @@ __all__ = [
 
 
 def _stream(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+    # The stream's handle without the Stream object around it (2 us a call).
+    return torch._C._cuda_getCurrentRawStream(
+        torch.cuda.current_device() if dev.index is None else dev.index)
+
+
+class _SameDevice:
+    """Stands in for torch.cuda.device(dev) where dev is current already."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_SAME_DEVICE = _SameDevice()
+
+
+def _on(dev: torch.device):
+    """Context in which dev is the current CUDA device (a launch needs that)."""
+    return _SAME_DEVICE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 def _p(t: Optional[torch.Tensor]):
@@ -175,7 +195,7 @@ def router_group_topk(logits: torch.Tensor, k: int, score: str = "sigmoid", num_
         ti = torch.empty((t, k), dtype=torch.int64, device=dev)
     rmap = torch.empty((t, e), dtype=torch.bool, device=dev)
     probs = torch.empty((t, e), dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
+    with _on(dev):
         _lib.call("moe_router_group_topk", _p(lg), _p(bias), t, e, int(k),
                   1 if score == "softmax" else 2, int(num_groups), int(topk_groups),
                   1 if group_score == "top2" else 0, 1 if renorm else 0, float(scale), _p(tv),
@@ -227,7 +247,7 @@ def router_topk_backward(logits: torch.Tensor, topk_idx: torch.Tensor,
     lg, ix, gv, gp, b, pl = (None if v is None else v.contiguous()
                              for v in (logits, topk_idx, grad_vals, grad_probs, bias, placement))
     out = torch.empty((t, e), dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
+    with _on(dev):
         _lib.call("moe_router_topk_backward", _p(lg), _p(b), _p(pl), _p(ix), _p(gv), _p(gp), t, e,
                   k, modes[score], 1 if renorm else 0, float(scale), _p(out), _stream(dev))
     return out
