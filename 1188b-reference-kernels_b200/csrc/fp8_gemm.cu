@@ -9,11 +9,23 @@
 // 32-bit cell per row holding the bytes of four consecutive 128-blocks; the
 // instruction descriptor selects the byte (k-block index & 3).
 //
-// One persistent CTA per SM, 224 threads:
-//   warp 0     TMA producer: 128 x 128 A tile and two 128 x 128 B tiles (48 KB) per stage and 128-block of K
-//   warp 1     TMEM owner; one thread copies scales to TMEM (tcgen05.cp) and issues the MMAs (M=128, N=256, K=32)
+// Two forms of one kernel, persistent, 224 threads a CTA:
+//   pair    clusters of two CTAs (cta_group::2) on 256 x 256 tiles, for groups of at least 256 rows: each CTA
+//           stages its own 128 A rows and half of the B tile (32 KB a 128-block of K, six stages), the leader
+//           issues M=256, N=256 MMAs over both shared memories into both TMEMs
+//   single  128 x 256 tiles (48 KB a 128-block, four stages) for smaller groups, where the weight stream is
+//           what takes the time
+// Warps:
+//   warp 0     TMA producer
+//   warp 1     TMEM owner; copies scales to TMEM (tcgen05.cp) and issues the MMAs (K=32)
 //   warps 2-5  epilogue, one row per thread
-//   warp 6     scales: global memory -> shared memory in the layout of tcgen05.cp, one 512-deep K group ahead
+//   warp 6     scales: global memory -> shared memory in the layout of tcgen05.cp, ahead of the MMAs. Every CTA
+//              keeps the scales of its own 128 rows and of all 256 columns
+// TMEM: two accumulators of 256 columns and two scale buffers of 12 would need
+// 536 of 512 columns, so accumulator 1 starts at column 224 and the two share
+// the 32 columns 224..255. The epilogue reads those first and hands them over
+// on a barrier of their own (`shared`), which the next tile's MMAs wait for;
+// the rest of a tile's epilogue overlaps the next tile's mainloop.
 // Rows are described by the group table of moe_grouped_gemm_plan_*. Every
 // wait is bounded (2 s): on timeout the kernel records an error word, drains
 // its copies and MMAs, frees TMEM and returns.
@@ -32,19 +44,29 @@ using gg::Tile;
 using gg::raise_abort;
 using gg::wait_drain;
 
-constexpr int BM = 128;
 constexpr int BN = 256;
-constexpr int kStages = 4;
 constexpr int kThreads = 224;
-constexpr uint32_t kTileBytes = 128 * 128;             // 128 rows (or reduction rows) x 128 bytes
-constexpr uint32_t kStageBytes = 3 * kTileBytes;       // A, B columns 0..127, B columns 128..255
-constexpr int kSfStages = 6;                           // scale buffers in shared memory
-constexpr int kSfTmem = 2;                             // and in TMEM
-constexpr int kSfBatch = 4;                            // K groups whose scales are loaded at once
-constexpr uint32_t kSfBytes = 512 + 1024;              // 128 A rows and 256 B rows, one 32-bit cell each
-constexpr size_t kSmemBytes = 1024 + kStages * kStageBytes + kSfStages * kSfBytes + 512;
+constexpr uint32_t kTileBytes = 128 * 128;  // 128 rows (or reduction rows) x 128 bytes
+constexpr int kFewRows = 32;   // single CTA: M-tiles of at most so many rows load a box of that height
+constexpr int kSfStages = 6;   // scale buffers in shared memory
+constexpr int kSfTmem = 2;     // and in TMEM
+constexpr int kSfBatch = 4;    // K groups whose scales are loaded at once
+constexpr uint32_t kSfBytes = 512 + 1024;    // 128 A rows and 256 B rows, one 32-bit cell each
+constexpr uint32_t kEpiWarpBytes = 4096;     // per epilogue warp: two 32 x 64-byte boxes or one 32 x 128-byte box
+
+template <bool kPair>
+struct Shape {
+  static constexpr int kTileM = kPair ? 256 : 128;
+  static constexpr int kStages = kPair ? 6 : 4;
+  static constexpr uint32_t kStageBytes = (kPair ? 2 : 3) * kTileBytes;  // of one CTA: A, half of B or all
+  static constexpr size_t kSmemBytes =
+      1024 + kStages * kStageBytes + 4 * kEpiWarpBytes + kSfStages * kSfBytes + 512;
+  static_assert(kSmemBytes <= 232448, "shared memory per CTA");
+};
+
 constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kSfCol = 480;                       // TMEM columns of the scales: 4 for A, 8 for B per stage
+constexpr uint32_t kAccCol1 = 224;  // first column of accumulator 1
+constexpr uint32_t kSfCol = 480;    // TMEM columns of the scales: 4 for A, 8 for B per buffer
 
 constexpr int64_t kSlabBytes = 32ll << 20;  // weight bytes walked per pass: they stay in L2 beside the rows
 
@@ -120,13 +142,23 @@ MOE_DEVICE void umma_mxf8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uin
 MOE_DEVICE uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
 MOE_DEVICE bool all_lanes(bool v) { return __all_sync(0xffffffffu, v) != 0; }
 
+// Tile load into this CTA's shared memory; a pair counts the bytes on the
+// leader's barrier.
+template <bool kPair>
 MOE_DEVICE void tma_load_3d(uint32_t dst, const void* tmap, int32_t x, int32_t y, int32_t z,
-                            uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(bar)
-      : "memory");
+                            uint32_t bar, uint64_t policy) {
+  if constexpr (kPair)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        ".L2::cache_hint [%0], [%1, {%2, %3, %4}], [%5], %6;" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(bar), "l"(policy)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        ".L2::cache_hint [%0], [%1, {%2, %3, %4}], [%5], %6;" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(bar), "l"(policy)
+        : "memory");
 }
 
 // Four scale bytes kb0..kb0+3 of a row of `num_kb` bytes at p (1.0 past its
@@ -162,391 +194,6 @@ MOE_DEVICE void load_scale_cells(const Params& p, int64_t row0, int64_t wi, int 
   }
 }
 
-__global__ void __launch_bounds__(kThreads, 1)
-    grouped_gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_a,
-                            const __grid_constant__ CUtensorMap tmap_b, const Params p) {
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t raw_addr = smem_u32(smem_raw);
-  const uint32_t base = (raw_addr + 1023u) & ~1023u;
-  uint8_t* base_ptr = smem_raw + (base - raw_addr);
-  uint8_t* sf_ptr = base_ptr + kStages * kStageBytes;
-  const uint32_t sf_base = base + kStages * kStageBytes;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sf_ptr + kSfStages * kSfBytes);
-  const uint32_t bar0 = smem_u32(bars);
-  auto full_bar = [&](int s) { return bar0 + 8u * s; };
-  auto empty_bar = [&](int s) { return bar0 + 8u * (kStages + s); };
-  auto sf_full = [&](int s) { return bar0 + 8u * (2 * kStages + s); };
-  auto sf_empty = [&](int s) { return bar0 + 8u * (2 * kStages + kSfStages + s); };
-  auto sf_used = [&](int b) { return bar0 + 8u * (2 * kStages + 2 * kSfStages + b); };
-  const uint32_t acc_full = bar0 + 8u * (2 * kStages + 2 * kSfStages + kSfTmem);
-  const uint32_t acc_empty = acc_full + 8u;
-  const uint32_t drain_bar = acc_full + 16u;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kStages + 2 * kSfStages + kSfTmem + 3);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-
-  const int warp = static_cast<int>(uniform(static_cast<uint32_t>(warp_id())));
-  const int lane = lane_id();
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
-      mbar_init(full_bar(s), 1);
-      mbar_init(empty_bar(s), 1);
-    }
-    for (int s = 0; s < kSfStages; ++s) {
-      mbar_init(sf_full(s), 1);
-      mbar_init(sf_empty(s), 1);
-    }
-    for (int b = 0; b < kSfTmem; ++b) mbar_init(sf_used(b), 1);
-    mbar_init(acc_full, 1);
-    mbar_init(acc_empty, 4);
-    mbar_init(drain_bar, 1);
-    *abort_flag = 0;
-    fence_mbar_init();
-  }
-  if (warp == 0 && lane == 0) {
-    tma_prefetch_desc(&tmap_a);
-    tma_prefetch_desc(&tmap_b);
-  }
-  if (warp == 1) {
-    tmem_alloc(smem_u32(tmem_slot), kTmemCols);
-    tmem_relinquish();
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = uniform(*tmem_slot);
-  const int groups4 = (p.num_kb + 3) / 4;  // 512-deep K groups, one scale cell each
-
-  gg::WalkerRT<BM> walker{p.rows, p.G, p.n_tiles, 1 << 20, 0};
-  Tile tile;
-
-  if (warp == 0) {
-    // ---------------------------------------------------------------- producer
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      int issued[kStages];
-#pragma unroll
-      for (int s = 0; s < kStages; ++s) issued[s] = -1;
-      bool ok = true;
-      for (long long t = blockIdx.x; ok && walker.locate(t, tile); t += gridDim.x) {
-        const int row0 = p.row_start[tile.g] + tile.m_idx * BM;
-        const int wi = p.widx[tile.g];
-        const int n0 = p.epilogue == 1 ? tile.n_idx * 128 : tile.n_idx * BN;
-        const int n1 = p.epilogue == 1 ? p.f_half + n0 : n0 + 128;
-        for (int kb = 0; kb < p.num_kb; ++kb) {
-          if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag)) {
-            ok = false;
-            break;
-          }
-          const uint32_t sa = base + stage * kStageBytes;
-          mbar_arrive_expect_tx(full_bar(stage), kStageBytes);
-          tma_load_3d(sa, &tmap_a, kb * 128, row0, 0, full_bar(stage));
-          if (p.b_mn) {
-            tma_load_3d(sa + kTileBytes, &tmap_b, n0, kb * 128, wi, full_bar(stage));
-            tma_load_3d(sa + 2 * kTileBytes, &tmap_b, n1, kb * 128, wi, full_bar(stage));
-          } else {
-            tma_load_3d(sa + kTileBytes, &tmap_b, kb * 128, n0, wi, full_bar(stage));
-            tma_load_3d(sa + 2 * kTileBytes, &tmap_b, kb * 128, n1, wi, full_bar(stage));
-          }
-          issued[stage] = static_cast<int>(phase);
-          if (++stage == kStages) {
-            stage = 0;
-            phase ^= 1u;
-          }
-        }
-      }
-      if (!ok) {
-        raise_abort(abort_flag, p.err, kErrProducer);
-        for (int s = 0; s < kStages; ++s)
-          if (issued[s] >= 0) wait_drain(full_bar(s), static_cast<uint32_t>(issued[s]));
-      }
-    }
-    __syncwarp();
-  } else if (warp == 1) {
-    // ---------------------------------------------------------------- MMA issuer
-    // The whole warp runs the loop in step (every wait's answer is a vote) and
-    // one lane issues: the operands of an MMA are then warp-uniform registers.
-    // With the loop in one lane's branch an MMA took 240 clocks to issue,
-    // against the unit's own 128.
-    {
-      const bool issuer = lane == 0;
-      const uint32_t idesc = idesc_mxf8(BM, BN, p.b_mn != 0);
-      // +32 values along K: 32 bytes inside a K-major swizzle row; 32 reduction
-      // rows (four 1024-byte groups of 8) of an MN-major tile.
-      const uint64_t bstep = p.b_mn ? 4096ull >> 4 : 32ull >> 4;
-      int stage = 0, sf = 0, copied = 0, used = 0;
-      uint32_t phase = 0, sf_phase = 0, acc_phase = 0;
-      bool ok = true, issued_any = false, ready = false;
-      // Scales of the next K group (the CTA's groups in order, across tiles) to the
-      // TMEM buffer that the group before the current one has used. Called in
-      // the middle of a group, so that neither wait is for work just issued.
-      auto copy_scales = [&]() {
-        const uint32_t b = static_cast<uint32_t>(copied & 1);
-        if (!all_lanes(mbar_wait(sf_used(b), static_cast<uint32_t>((copied >> 1) & 1) ^ 1u, abort_flag) &&
-                       mbar_wait(sf_full(sf), sf_phase, abort_flag)))
-          return false;
-        tc_fence_after();
-        const uint32_t sfa = tmem + kSfCol + b * 12u;
-        const uint32_t src = sf_base + static_cast<uint32_t>(sf) * kSfBytes;
-        if (issuer) {
-          tmem_copy_scales(sfa, sf_desc(src));
-          tmem_copy_scales(sfa + 4u, sf_desc(src + 512u));
-          tmem_copy_scales(sfa + 8u, sf_desc(src + 1024u));
-          umma_commit(sf_empty(sf));
-        }
-        __syncwarp();
-        issued_any = true;
-        ++copied;
-        if (++sf == kSfStages) {
-          sf = 0;
-          sf_phase ^= 1u;
-        }
-        return true;
-      };
-      long long t = blockIdx.x;
-      bool more = all_lanes(walker.locate(t, tile));
-      if (more) ok = copy_scales();
-      while (ok && more) {
-        t += gridDim.x;
-        more = all_lanes(walker.locate(t, tile));  // whether another tile follows
-        if (!all_lanes(mbar_wait(acc_empty, acc_phase ^ 1u, abort_flag))) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        for (int kg = 0; kg < groups4 && ok; ++kg, ++used) {
-          const uint32_t sfa = tmem + kSfCol + static_cast<uint32_t>(used & 1) * 12u;
-          const int n = min(4, p.num_kb - kg * 4);
-          for (int i = 0; i < n; ++i) {
-            if (!ready && !all_lanes(mbar_wait(full_bar(stage), phase, abort_flag))) {
-              ok = false;
-              break;
-            }
-            // the next stage is looked at before this one's MMAs are issued,
-            // so that the answer's latency does not stand between the two
-            const int next = stage + 1 == kStages ? 0 : stage + 1;
-            ready = all_lanes(mbar_try_wait(full_bar(next), next == 0 ? phase ^ 1u : phase));
-            tc_fence_after();
-            const uint32_t sa = base + stage * kStageBytes;
-            const uint64_t ad = umma_desc_k_sw128(sa);
-            const uint64_t bd = p.b_mn ? umma_desc_mn_sw128(sa + kTileBytes, kTileBytes)
-                                       : umma_desc_k_sw128(sa + kTileBytes);
-            const uint32_t id = with_sf_id(idesc, static_cast<uint32_t>(i));
-            if (issuer) {
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                umma_mxf8(tmem, ad + 2ull * k, bd + bstep * k, id, sfa, sfa + 4u,
-                      (kg | i | k) != 0 ? 1u : 0u);
-              umma_commit(empty_bar(stage));
-            }
-            __syncwarp();
-            if (++stage == kStages) {
-              stage = 0;
-              phase ^= 1u;
-            }
-            if (i == min(1, n - 1) && (kg + 1 < groups4 || more) && !copy_scales()) {
-              ok = false;
-              break;
-            }
-          }
-          if (!ok) break;
-          if (issuer) umma_commit(sf_used(used & 1));
-        }
-        if (!ok) break;
-        if (issuer) umma_commit(acc_full);
-        acc_phase ^= 1u;
-      }
-      if (!ok && issuer) {
-        raise_abort(abort_flag, p.err, kErrMma);
-        if (issued_any) {
-          umma_commit(drain_bar);
-          wait_drain(drain_bar, 0);
-        }
-      }
-    }
-    __syncwarp();
-  } else if (warp == 6) {
-    // ---------------------------------------------------------------- scales
-    int sf = 0;
-    uint32_t sf_phase = 0;
-    bool ok = true;
-    for (long long t = blockIdx.x; ok && walker.locate(t, tile); t += gridDim.x) {
-      const int64_t row0 = static_cast<int64_t>(p.row_start[tile.g]) + tile.m_idx * BM;
-      const int64_t wi = p.widx[tile.g];
-      const int nb0 = p.epilogue == 1 ? tile.n_idx : tile.n_idx * 2;
-      const int nb1 = p.epilogue == 1 ? p.f_half / 128 + tile.n_idx : nb0 + 1;
-      for (int kg0 = 0; kg0 < groups4 && ok; kg0 += kSfBatch) {
-        uint32_t a[kSfBatch][4], b[kSfBatch][2];
-#pragma unroll
-        for (int j = 0; j < kSfBatch; ++j)
-          if (kg0 + j < groups4) load_scale_cells(p, row0, wi, nb0, nb1, kg0 + j, lane, a[j], b[j]);
-#pragma unroll
-        for (int j = 0; j < kSfBatch; ++j) {
-          if (kg0 + j >= groups4) break;
-          if (!mbar_wait(sf_empty(sf), sf_phase ^ 1u, abort_flag)) {
-            ok = false;
-            break;
-          }
-          uint4* dst = reinterpret_cast<uint4*>(sf_ptr + sf * kSfBytes) + lane;
-          dst[0] = make_uint4(a[j][0], a[j][1], a[j][2], a[j][3]);
-          dst[32] = make_uint4(b[j][0], b[j][0], b[j][0], b[j][0]);
-          dst[64] = make_uint4(b[j][1], b[j][1], b[j][1], b[j][1]);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(sf_full(sf));
-          if (++sf == kSfStages) {
-            sf = 0;
-            sf_phase ^= 1u;
-          }
-        }
-      }
-    }
-    if (!ok && lane == 0) raise_abort(abort_flag, p.err, kErrScales);
-    __syncwarp();
-  } else {
-    // ---------------------------------------------------------------- epilogue
-    const int quad = warp & 3;  // TMEM lanes 32*quad .. of this warp
-    uint32_t acc_phase = 0;
-    bool ok = true;
-    for (long long t = blockIdx.x; walker.locate(t, tile); t += gridDim.x) {
-      if (!mbar_wait(acc_full, acc_phase, abort_flag)) {
-        ok = false;
-        break;
-      }
-      acc_phase ^= 1u;
-      tc_fence_after();
-      const int m_local = tile.m_idx * BM + quad * 32 + lane;
-      const int64_t row = static_cast<int64_t>(p.row_start[tile.g]) + m_local;
-      const bool rvalid = m_local < p.rows[tile.g] && row < p.x_rows;
-      const uint32_t tbase = tmem + (static_cast<uint32_t>(quad * 32) << 16);
-      if (p.epilogue == 0) {
-        const int n0 = tile.n_idx * BN;
-        __nv_bfloat16* orow = static_cast<__nv_bfloat16*>(p.out) + row * p.n;
-#pragma unroll 1
-        for (int c = 0; c < BN / 32; ++c) {
-          uint32_t r[32];
-          tmem_ld_32x32b_x32(tbase + c * 32, r);
-          tmem_ld_wait();
-          if (rvalid) {
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-              const int col = n0 + c * 32 + v * 8;
-              if (col + 8 <= p.n) {
-                uint32_t o[4];
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                  o[q] = pack_bf16x2(__uint_as_float(r[v * 8 + 2 * q]),
-                                     __uint_as_float(r[v * 8 + 2 * q + 1]));
-                *reinterpret_cast<uint4*>(orow + col) = make_uint4(o[0], o[1], o[2], o[3]);
-              }
-            }
-          }
-        }
-      } else {
-        // gate in columns 0..127, up in 128..255; the 128 results of a row
-        // are one block of the quantised output
-        float h[128];
-        float amax = 0.f;
-        __nv_bfloat16* prow = p.pre == nullptr ? nullptr : p.pre + row * p.n + tile.n_idx * 128;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t gr[32], ur[32];
-          tmem_ld_32x32b_x32(tbase + c * 32, gr);
-          tmem_ld_32x32b_x32(tbase + 128 + c * 32, ur);
-          tmem_ld_wait();
-#pragma unroll
-          for (int q = 0; q < 16; ++q) {
-            const float2 v = swiglu2_f32(
-                make_float2(__uint_as_float(gr[2 * q]), __uint_as_float(gr[2 * q + 1])),
-                make_float2(__uint_as_float(ur[2 * q]), __uint_as_float(ur[2 * q + 1])));
-            h[c * 32 + 2 * q] = v.x;
-            h[c * 32 + 2 * q + 1] = v.y;
-            amax = fmaxf(amax, fmaxf(fp8::finite_abs(v.x), fp8::finite_abs(v.y)));
-          }
-          if (prow != nullptr && rvalid) {
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-              uint32_t o[4], u[4];
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                o[q] = pack_bf16x2(__uint_as_float(gr[v * 8 + 2 * q]),
-                                   __uint_as_float(gr[v * 8 + 2 * q + 1]));
-                u[q] = pack_bf16x2(__uint_as_float(ur[v * 8 + 2 * q]),
-                                   __uint_as_float(ur[v * 8 + 2 * q + 1]));
-              }
-              *reinterpret_cast<uint4*>(prow + c * 32 + v * 8) = make_uint4(o[0], o[1], o[2], o[3]);
-              *reinterpret_cast<uint4*>(prow + p.f_half + c * 32 + v * 8) =
-                  make_uint4(u[0], u[1], u[2], u[3]);
-            }
-          }
-        }
-        if (rvalid) {
-          const uint32_t sb = fp8::scale_byte(amax);
-          const float inv = fp8::inverse_scale(sb);
-          uint4* orow = reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) + row * p.f_half +
-                                                 tile.n_idx * 128);
-#pragma unroll
-          for (int v = 0; v < 8; ++v) {
-            uint32_t o[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const int j = v * 16 + q * 4;
-              o[q] = fp8::pack4(fp8::scaled(h[j], inv), fp8::scaled(h[j + 1], inv),
-                                fp8::scaled(h[j + 2], inv), fp8::scaled(h[j + 3], inv));
-            }
-            orow[v] = make_uint4(o[0], o[1], o[2], o[3]);
-          }
-          p.out_scale[row * (p.f_half / 128) + tile.n_idx] = static_cast<uint8_t>(sb);
-        }
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(acc_empty);
-    }
-    if (!ok && lane == 0) raise_abort(abort_flag, p.err, kErrEpilogue);
-  }
-
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 1) {
-    tc_fence_after();
-    tmem_dealloc(tmem, kTmemCols);
-  }
-}
-
-// ---------------------------------------------------------------------------
-// CTA-pair kernel (tcgen05 cta_group::2, clusters of 2): groups of at least
-// 256 rows, 256 x 256 tiles. Each CTA stages its own 128 A rows and half of
-// the B tile (32 KB a 128-block, six stages); the leader issues M=256, N=256
-// MMAs that read both CTAs' shared memory and scales and fill both TMEMs.
-// Every CTA keeps the scales of its own rows and of all 256 columns.
-//
-// TMEM: two accumulators of 256 columns and two scale buffers of 12 need 536
-// of 512 columns, so accumulator 1 starts at column 224 and the two share the
-// 32 columns 224..255. The epilogue reads those first and hands them over on
-// a barrier of their own (`shared`), which the next tile's MMAs wait for; the
-// rest of a tile's epilogue overlaps the next tile's mainloop.
-// ---------------------------------------------------------------------------
-namespace pairk {
-constexpr int kTileM = 256;
-constexpr int kStages = 6;
-constexpr uint32_t kStageBytes = 2 * kTileBytes;
-constexpr uint32_t kAccCol1 = 224;
-constexpr uint32_t kEpiWarpBytes = 4096;  // per epilogue warp: two 32 x 64-byte boxes or one 32 x 128-byte box
-constexpr size_t kSmemBytes =
-    1024 + kStages * kStageBytes + 4 * kEpiWarpBytes + kSfStages * kSfBytes + 512;
-static_assert(kSmemBytes <= 232448, "shared memory per CTA");
-}  // namespace pairk
-
-MOE_DEVICE void tma_load_3d_pair(uint32_t dst, const void* tmap, int32_t x, int32_t y, int32_t z,
-                                 uint32_t bar_cluster) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(bar_cluster)
-      : "memory");
-}
-
 MOE_DEVICE void tmem_copy_scales_pair(uint32_t taddr, uint64_t desc) {
   asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc)
                : "memory");
@@ -569,14 +216,62 @@ MOE_DEVICE void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, 
                : "memory");
 }
 
+// What the two forms do differently around the same instruction.
+template <bool kPair>
+struct Op {
+  static MOE_DEVICE bool wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+    if constexpr (kPair) return mbar_wait_cluster(bar, parity, abort_flag);
+    return mbar_wait(bar, parity, abort_flag);
+  }
+  // a commit that both CTAs see / that the issuing CTA alone needs
+  static MOE_DEVICE void commit(uint32_t bar) {
+    if constexpr (kPair)
+      umma_commit_pair(bar, 0x3);
+    else
+      umma_commit(bar);
+  }
+  static MOE_DEVICE void commit_own(uint32_t bar) {
+    if constexpr (kPair)
+      umma_commit_pair(bar, 0x1);
+    else
+      umma_commit(bar);
+  }
+  static MOE_DEVICE uint32_t leader(uint32_t bar) {
+    if constexpr (kPair) return map_to_rank(bar, 0);
+    return bar;
+  }
+  static MOE_DEVICE void arrive(uint32_t leader_bar) {
+    if constexpr (kPair)
+      mbar_arrive_cluster(leader_bar);
+    else
+      mbar_arrive(leader_bar);
+  }
+  static MOE_DEVICE void copy_scales(uint32_t taddr, uint64_t desc) {
+    if constexpr (kPair)
+      tmem_copy_scales_pair(taddr, desc);
+    else
+      tmem_copy_scales(taddr, desc);
+  }
+  static MOE_DEVICE void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa,
+                             uint32_t sfb, uint32_t accumulate) {
+    if constexpr (kPair)
+      umma_mxf8_pair(d, a, b, idesc, sfa, sfb, accumulate);
+    else
+      umma_mxf8(d, a, b, idesc, sfa, sfb, accumulate);
+  }
+};
+
+template <bool kPair>
 __global__ void __launch_bounds__(kThreads, 1)
-    grouped_gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a,
-                                 const __grid_constant__ CUtensorMap tmap_b,
-                                 const __grid_constant__ CUtensorMap tmap_out,
-                                 const __grid_constant__ CUtensorMap tmap_pre, const Params p) {
-  using namespace pairk;
-  constexpr int kS = pairk::kStages;
-  constexpr uint32_t kSB = pairk::kStageBytes;
+    grouped_gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_a,
+                            const __grid_constant__ CUtensorMap tmap_a_few,
+                            const __grid_constant__ CUtensorMap tmap_b,
+                            const __grid_constant__ CUtensorMap tmap_out,
+                            const __grid_constant__ CUtensorMap tmap_pre, const Params p) {
+  using O = Op<kPair>;
+  constexpr int kTileM = Shape<kPair>::kTileM;
+  constexpr int kS = Shape<kPair>::kStages;
+  constexpr uint32_t kSB = Shape<kPair>::kStageBytes;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t base = (raw_addr + 1023u) & ~1023u;
@@ -598,10 +293,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kS + 2 * kSfStages + kSfTmem + 6);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const uint32_t rank = cluster_ctarank();
+  const uint32_t rank = kPair ? cluster_ctarank() : 0u;
   const bool leader = rank == 0;
-  const long long cid = cluster_id_x();
-  const long long ncl = num_clusters_x();
+  const long long cid = kPair ? cluster_id_x() : blockIdx.x;
+  const long long ncl = kPair ? num_clusters_x() : gridDim.x;
   const int warp = static_cast<int>(uniform(static_cast<uint32_t>(warp_id())));
   const int lane = lane_id();
   if (threadIdx.x == 0) {
@@ -610,15 +305,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(empty_bar(s), 1);
     }
     for (int s = 0; s < kSfStages; ++s) {
-      mbar_init(sf_full(s), 2);  // the scale warps of both CTAs
+      mbar_init(sf_full(s), kPair ? 2 : 1);  // the scale warp of each CTA
       mbar_init(sf_empty(s), 1);
     }
     for (int b = 0; b < kSfTmem; ++b) mbar_init(sf_used(b), 1);
     for (int a = 0; a < 2; ++a) {
       mbar_init(acc_full(a), 1);
-      mbar_init(acc_empty(a), 8);  // four epilogue warps in each CTA
+      mbar_init(acc_empty(a), kPair ? 8 : 4);  // four epilogue warps in each CTA
     }
-    mbar_init(shared_bar, 8);
+    mbar_init(shared_bar, kPair ? 8 : 4);
     mbar_init(drain_bar, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -628,12 +323,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&tmap_b);
   }
   if (warp == 1) {
-    tmem_alloc_pair(smem_u32(tmem_slot), kTmemCols);
-    tmem_relinquish_pair();
+    if constexpr (kPair) {
+      tmem_alloc_pair(smem_u32(tmem_slot), kTmemCols);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(smem_u32(tmem_slot), kTmemCols);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
   __syncthreads();
-  cluster_sync();  // barriers of both CTAs initialised before any remote use
+  if constexpr (kPair) cluster_sync();  // barriers of both CTAs initialised before any remote use
   tc_fence_after();
   const uint32_t tmem = uniform(*tmem_slot);
   const int groups4 = (p.num_kb + 3) / 4;
@@ -653,21 +353,36 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (long long t = cid; ok && walker.locate(t, tile); t += ncl) {
         const int row0 = p.row_start[tile.g] + tile.m_idx * kTileM + static_cast<int>(rank) * 128;
         const int wi = p.widx[tile.g];
-        const int n0 = p.epilogue == 1 ? tile.n_idx * 128 + static_cast<int>(rank) * p.f_half
-                                       : tile.n_idx * BN + static_cast<int>(rank) * 128;
+        // first weight row (KN: column) of the two halves of the B tile; a
+        // pair's CTA loads its own
+        const int n0 = p.epilogue == 1 ? tile.n_idx * 128 : tile.n_idx * BN;
+        const int n1 = p.epilogue == 1 ? p.f_half + n0 : n0 + 128;
+        const int rows = p.rows[tile.g];
+        // A tile with few rows loads only those (the others keep what an
+        // earlier tile left there: an MMA row depends on no other).
+        const bool few = !kPair && rows - tile.m_idx * kTileM <= kFewRows;
+        const CUtensorMap* map_a = few ? &tmap_a_few : &tmap_a;
+        const uint32_t bytes = kPair ? 2 * kSB : few ? kSB - (128 - kFewRows) * 128u : kSB;
+        // A weight that one M-tile reads is not read again: it leaves L2
+        // first (32 groups of 100 rows, K 2048: 122 -> 114 us).
+        const uint64_t policy =
+            !kPair && rows <= kTileM ? l2_policy_evict_first() : l2_policy_evict_normal();
         for (int kb = 0; kb < p.num_kb; ++kb) {
           if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag)) {
             ok = false;
             break;
           }
           const uint32_t sa = base + stage * kSB;
-          const uint32_t leader_full = map_to_rank(full_bar(stage), 0);
-          if (leader) mbar_arrive_expect_tx(full_bar(stage), 2 * kSB);
-          tma_load_3d_pair(sa, &tmap_a, kb * 128, row0, 0, leader_full);
-          if (p.b_mn)
-            tma_load_3d_pair(sa + kTileBytes, &tmap_b, n0, kb * 128, wi, leader_full);
-          else
-            tma_load_3d_pair(sa + kTileBytes, &tmap_b, kb * 128, n0, wi, leader_full);
+          const uint32_t leader_full = O::leader(full_bar(stage));
+          if (leader) mbar_arrive_expect_tx(full_bar(stage), bytes);
+          tma_load_3d<kPair>(sa, map_a, kb * 128, row0, 0, leader_full, l2_policy_evict_normal());
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (kPair && h != static_cast<int>(rank)) continue;
+            const int n = h ? n1 : n0;
+            tma_load_3d<kPair>(sa + (kPair ? 1 : 1 + h) * kTileBytes, &tmap_b, p.b_mn ? n : kb * 128,
+                               p.b_mn ? kb * 128 : n, wi, leader_full, policy);
+          }
           issued[stage] = static_cast<int>(phase);
           if (++stage == kS) {
             stage = 0;
@@ -702,7 +417,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (leader) {
       const bool issuer = lane == 0;
       const uint32_t idesc = idesc_mxf8(kTileM, BN, p.b_mn != 0);
-      const uint64_t bstep = p.b_mn ? 4096ull >> 4 : 32ull >> 4;  // see grouped_gemm_fp8_kernel
+      // +32 values along K: 32 bytes inside a K-major swizzle row; 32 reduction
+      // rows (four 1024-byte groups of 8) of an MN-major tile.
+      const uint64_t bstep = p.b_mn ? 4096ull >> 4 : 32ull >> 4;
       int stage = 0, sf = 0, copied = 0, used = 0, it = 0;
       uint32_t phase = 0, sf_phase = 0;
       bool ok = true, issued_any = false, ready = false;
@@ -712,16 +429,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto copy_scales = [&]() {
         const uint32_t b = static_cast<uint32_t>(copied & 1);
         if (!all_lanes(mbar_wait(sf_used(b), static_cast<uint32_t>((copied >> 1) & 1) ^ 1u, abort_flag) &&
-                       mbar_wait_cluster(sf_full(sf), sf_phase, abort_flag)))
+                       O::wait(sf_full(sf), sf_phase, abort_flag)))
           return false;
         tc_fence_after();
         const uint32_t sfa = tmem + kSfCol + b * 12u;
         const uint32_t src = sf_base + static_cast<uint32_t>(sf) * kSfBytes;
         if (issuer) {
-          tmem_copy_scales_pair(sfa, sf_desc(src));
-          tmem_copy_scales_pair(sfa + 4u, sf_desc(src + 512u));
-          tmem_copy_scales_pair(sfa + 8u, sf_desc(src + 1024u));
-          umma_commit_pair(sf_empty(sf), 0x3);
+          O::copy_scales(sfa, sf_desc(src));
+          O::copy_scales(sfa + 4u, sf_desc(src + 512u));
+          O::copy_scales(sfa + 8u, sf_desc(src + 1024u));
+          O::commit(sf_empty(sf));
         }
         __syncwarp();
         issued_any = true;
@@ -743,8 +460,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         // the accumulator's last epilogue (two tiles ago) and the columns
         // shared with the other accumulator's (the last tile)
         if (!all_lanes(
-                mbar_wait_cluster(acc_empty(acc), static_cast<uint32_t>((it >> 1) & 1) ^ 1u, abort_flag) &&
-                mbar_wait_cluster(shared_bar, static_cast<uint32_t>(it & 1) ^ 1u, abort_flag))) {
+                O::wait(acc_empty(acc), static_cast<uint32_t>((it >> 1) & 1) ^ 1u, abort_flag) &&
+                O::wait(shared_bar, static_cast<uint32_t>(it & 1) ^ 1u, abort_flag))) {
           ok = false;
           break;
         }
@@ -770,9 +487,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (issuer) {
 #pragma unroll
               for (int k = 0; k < 4; ++k)
-                umma_mxf8_pair(d_tmem, ad + 2ull * k, bd + bstep * k, id, sfa, sfa + 4u,
+                O::mma(d_tmem, ad + 2ull * k, bd + bstep * k, id, sfa, sfa + 4u,
                       (kg | i | k) != 0 ? 1u : 0u);
-              umma_commit_pair(empty_bar(stage), 0x3);
+              O::commit(empty_bar(stage));
             }
             __syncwarp();
             if (++stage == kS) {
@@ -785,16 +502,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           if (!ok) break;
-          if (issuer) umma_commit_pair(sf_used(used & 1), 0x1);
+          if (issuer) O::commit_own(sf_used(used & 1));
         }
         if (!ok) break;
-        if (issuer) umma_commit_pair(acc_full(acc), 0x3);
+        if (issuer) O::commit(acc_full(acc));
         ++it;
       }
       if (!ok && issuer) {
         raise_abort(abort_flag, p.err, kErrMma);
         if (issued_any) {
-          umma_commit_pair(drain_bar, 0x1);
+          O::commit_own(drain_bar);
           wait_drain(drain_bar, 0);
         }
       }
@@ -821,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int j = 0; j < kSfBatch; ++j) {
           if (kg0 + j >= groups4) break;
-          if (!mbar_wait_cluster(sf_empty(sf), sf_phase ^ 1u, abort_flag)) {
+          if (!mbar_wait(sf_empty(sf), sf_phase ^ 1u, abort_flag)) {
             ok = false;
             break;
           }
@@ -831,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           dst[64] = make_uint4(b[j][1], b[j][1], b[j][1], b[j][1]);
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(map_to_rank(sf_full(sf), 0));
+          if (lane == 0) O::arrive(O::leader(sf_full(sf)));
           filled[sf] = static_cast<int>(sf_phase);
           if (++sf == kSfStages) {
             sf = 0;
@@ -851,16 +568,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // ---------------------------------------------------------------- epilogue (both CTAs)
     const int quad = warp & 3;
-    const uint32_t leader_empty0 = map_to_rank(acc_empty(0), 0);
-    const uint32_t leader_empty1 = map_to_rank(acc_empty(1), 0);
-    const uint32_t leader_shared = map_to_rank(shared_bar, 0);
+    const uint32_t leader_empty0 = O::leader(acc_empty(0));
+    const uint32_t leader_empty1 = O::leader(acc_empty(1));
+    const uint32_t leader_shared = O::leader(shared_bar);
     const uint32_t epi = epi_base + static_cast<uint32_t>(quad) * kEpiWarpBytes;
     uint32_t box_no = 0;
     int it = 0;
     bool ok = true;
     for (long long t = cid; walker.locate(t, tile); t += ncl, ++it) {
       const int acc = it & 1;
-      if (!mbar_wait_cluster(acc_full(acc), static_cast<uint32_t>((it >> 1) & 1), abort_flag)) {
+      if (!mbar_wait(acc_full(acc), static_cast<uint32_t>((it >> 1) & 1), abort_flag)) {
         ok = false;
         break;
       }
@@ -902,7 +619,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto release_shared = [&]() {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(leader_shared);
+        if (lane == 0) O::arrive(leader_shared);
       };
       if (p.epilogue == 0) {
         // accumulator 0 shares its last 32 columns, accumulator 1 its first
@@ -925,7 +642,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(acc ? leader_empty1 : leader_empty0);
+        if (lane == 0) O::arrive(acc ? leader_empty1 : leader_empty0);
       } else {
         // gate in columns 0..127, up in 128..255, 32 of each at a time; the
         // shared columns lie in the chunk that comes first. h[] is indexed in
@@ -948,7 +665,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (i == 3) {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(acc ? leader_empty1 : leader_empty0);
+            if (lane == 0) O::arrive(acc ? leader_empty1 : leader_empty0);
           }
 #pragma unroll
           for (int q = 0; q < 16; ++q) {
@@ -1018,16 +735,20 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   tc_fence_before();
   __syncthreads();
-  cluster_sync();  // no CTA leaves while its partner may still touch its memory
+  if constexpr (kPair) cluster_sync();  // no CTA leaves while its partner may still touch its memory
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc_pair(tmem, kTmemCols);
+    if constexpr (kPair)
+      tmem_dealloc_pair(tmem, kTmemCols);
+    else
+      tmem_dealloc(tmem, kTmemCols);
   }
 }
 
-// 3-D tensor map over bytes [d2, d1, d0] (d0 contiguous), box 128 x 128 x 1,
+// 3-D tensor map over bytes [d2, d1, d0] (d0 contiguous), box 128 x box_rows x 1,
 // 128-byte swizzle; reads outside give zeros.
-int make_tmap(CUtensorMap* m, const void* ptr, uint64_t d0, uint64_t d1, uint64_t d2) {
+int make_tmap(CUtensorMap* m, const void* ptr, uint64_t d0, uint64_t d1, uint64_t d2,
+              uint32_t box_rows = 128u) {
   auto encode = gg::get_encode_fn();
   if (encode == nullptr) {
     set_last_error("grouped_gemm_fp8: cuTensorMapEncodeTiled unavailable");
@@ -1035,7 +756,7 @@ int make_tmap(CUtensorMap* m, const void* ptr, uint64_t d0, uint64_t d1, uint64_
   }
   cuuint64_t dims[3] = {d0, d1, d2};
   cuuint64_t strides[2] = {d0, d0 * d1};
-  cuuint32_t box[3] = {128u, 128u, 1u};
+  cuuint32_t box[3] = {128u, box_rows, 1u};
   cuuint32_t estr[3] = {1u, 1u, 1u};
   const CUresult r =
       encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(ptr), dims, strides, box, estr,
@@ -1079,18 +800,18 @@ int prepare_device(int dev, int* clusters) {
     *clusters = pairs[dev];
     return MOE_OK;
   }
-  MOE_CUDA_CALL(cudaFuncSetAttribute(grouped_gemm_fp8_kernel,
+  MOE_CUDA_CALL(cudaFuncSetAttribute(grouped_gemm_fp8_kernel<false>,
                                      cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     static_cast<int>(kSmemBytes)),
+                                     static_cast<int>(Shape<false>::kSmemBytes)),
                 "cudaFuncSetAttribute(grouped_gemm_fp8)");
-  MOE_CUDA_CALL(cudaFuncSetAttribute(grouped_gemm_fp8_pair_kernel,
+  MOE_CUDA_CALL(cudaFuncSetAttribute(grouped_gemm_fp8_kernel<true>,
                                      cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     static_cast<int>(pairk::kSmemBytes)),
+                                     static_cast<int>(Shape<true>::kSmemBytes)),
                 "cudaFuncSetAttribute(grouped_gemm_fp8_pair)");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * 74);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = pairk::kSmemBytes;
+  cfg.dynamicSmemBytes = Shape<true>::kSmemBytes;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
@@ -1099,7 +820,7 @@ int prepare_device(int dev, int* clusters) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   int n = 0;
-  if (cudaOccupancyMaxActiveClusters(&n, grouped_gemm_fp8_pair_kernel, &cfg) != cudaSuccess) n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, grouped_gemm_fp8_kernel<true>, &cfg) != cudaSuccess) n = 0;
   cudaGetLastError();  // clear a non-sticky error of the query
   if (dev >= 0 && dev < 64) {
     pairs[dev] = n;
@@ -1153,8 +874,11 @@ extern "C" int moe_grouped_gemm_fp8(const void* x, const void* x_scale, const vo
   int st = g8::prepare_device(dev, &clusters);
   if (st) return st;
 
-  CUtensorMap ta, tb;
+  CUtensorMap ta, taf, tb;
   st = g8::make_tmap(&ta, x, static_cast<uint64_t>(K), static_cast<uint64_t>(x_rows), 1);
+  if (st) return st;
+  st = g8::make_tmap(&taf, x, static_cast<uint64_t>(K), static_cast<uint64_t>(x_rows), 1,
+                     g8::kFewRows);
   if (st) return st;
   st = w_kn ? g8::make_tmap(&tb, w, static_cast<uint64_t>(N), static_cast<uint64_t>(K),
                             static_cast<uint64_t>(num_w))
@@ -1186,18 +910,18 @@ extern "C" int moe_grouped_gemm_fp8(const void* x, const void* x_scale, const vo
   p.epilogue = epilogue;
   p.x_words = p.num_kb % 4 == 0 && (reinterpret_cast<uintptr_t>(x_scale) & 3) == 0;
   p.w_words = !w_kn && p.num_kb % 4 == 0 && (reinterpret_cast<uintptr_t>(w_scale) & 3) == 0;
+  CUtensorMap to, tp;
+  st = g8::make_store_tmap(&to, out, static_cast<uint64_t>(epilogue == 1 ? p.f_half : p.n),
+                           static_cast<uint64_t>(x_rows), epilogue == 0);
+  if (st) return st;
+  tp = to;
+  if (pre != nullptr) {
+    st = g8::make_store_tmap(&tp, pre, static_cast<uint64_t>(N), static_cast<uint64_t>(x_rows), true);
+    if (st) return st;
+  }
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (clusters > 0) {
-    if (x_rows >= g8::pairk::kTileM) {  // fewer rows: no group has a whole pair tile
-      CUtensorMap to, tp;
-      st = g8::make_store_tmap(&to, out, static_cast<uint64_t>(epilogue == 1 ? p.f_half : p.n),
-                               static_cast<uint64_t>(x_rows), epilogue == 0);
-      if (st) return st;
-      tp = to;
-      if (pre != nullptr)
-        st = g8::make_store_tmap(&tp, pre, static_cast<uint64_t>(N), static_cast<uint64_t>(x_rows),
-                                 true);
-      if (st) return st;
+    if (x_rows >= g8::Shape<true>::kTileM) {  // fewer rows: no group has a whole pair tile
       g8::Params pb = p;
       pb.rows = l.rows_body;
       pb.n_chunk = static_cast<int>(
@@ -1205,7 +929,7 @@ extern "C" int moe_grouped_gemm_fp8(const void* x, const void* x_scale, const vo
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3(2 * clusters);
       cfg.blockDim = dim3(g8::kThreads);
-      cfg.dynamicSmemBytes = g8::pairk::kSmemBytes;
+      cfg.dynamicSmemBytes = g8::Shape<true>::kSmemBytes;
       cfg.stream = s;
       cudaLaunchAttribute attr[1];
       attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1214,13 +938,15 @@ extern "C" int moe_grouped_gemm_fp8(const void* x, const void* x_scale, const vo
       attr[0].val.clusterDim.z = 1;
       cfg.attrs = attr;
       cfg.numAttrs = 1;
-      MOE_CUDA_CALL(cudaLaunchKernelEx(&cfg, g8::grouped_gemm_fp8_pair_kernel, ta, tb, to, tp, pb),
-                    "grouped_gemm_fp8 pair launch");
+      MOE_CUDA_CALL(
+          cudaLaunchKernelEx(&cfg, g8::grouped_gemm_fp8_kernel<true>, ta, ta, tb, to, tp, pb),
+          "grouped_gemm_fp8 pair launch");
     }
     p.row_start = l.tail_start;
     p.rows = l.rows_tail;
   }
-  g8::grouped_gemm_fp8_kernel<<<num_sms(dev), g8::kThreads, g8::kSmemBytes, s>>>(ta, tb, p);
+  g8::grouped_gemm_fp8_kernel<false><<<num_sms(dev), g8::kThreads, g8::Shape<false>::kSmemBytes, s>>>(
+      ta, taf, tb, to, tp, p);
   MOE_CUDA_CHECK_LAUNCH("grouped_gemm_fp8 launch");
   return MOE_OK;
 }
