@@ -346,9 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0;
-      int issued[kS];
-#pragma unroll
-      for (int s = 0; s < kS; ++s) issued[s] = -1;
+      long long issued = 0;
       bool ok = true;
       for (long long t = cid; ok && walker.locate(t, tile); t += ncl) {
         const int row0 = p.row_start[tile.g] + tile.m_idx * kTileM + static_cast<int>(rank) * 128;
@@ -383,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tma_load_3d<kPair>(sa + (kPair ? 1 : 1 + h) * kTileBytes, &tmap_b, p.b_mn ? n : kb * 128,
                                p.b_mn ? kb * 128 : n, wi, leader_full, policy);
           }
-          issued[stage] = static_cast<int>(phase);
+          ++issued;
           if (++stage == kS) {
             stage = 0;
             phase ^= 1u;
@@ -392,13 +390,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (ok) {
         // every stage's release lands in this CTA's shared memory: wait for the last ones
-        for (int s = 0; s < kS; ++s)
-          if (issued[s] >= 0) wait_drain(empty_bar(s), static_cast<uint32_t>(issued[s]));
+        for (long long i = issued > kS ? issued - kS : 0; i < issued; ++i)
+          wait_drain(empty_bar(static_cast<int>(i % kS)), static_cast<uint32_t>(i / kS) & 1u);
       } else {
         raise_abort(abort_flag, p.err, kErrProducer);
         if (leader) {
-          for (int s = 0; s < kS; ++s)
-            if (issued[s] >= 0) wait_drain(full_bar(s), static_cast<uint32_t>(issued[s]));
+          for (long long i = issued > kS ? issued - kS : 0; i < issued; ++i)
+            wait_drain(full_bar(static_cast<int>(i % kS)), static_cast<uint32_t>(i / kS) & 1u);
         } else {
           // copies count on the leader's barrier; give them a bounded time to land
           const unsigned long long t0 = globaltimer_ns();

@@ -502,6 +502,9 @@ class MoELayerEP:
         no data and never wait on each other on the device. The output is the
         same, bit for bit, as with C = 1 (same receive rows, same GEMM
         groups, same combine)."""
+        if not isinstance(local_weights, MoEWeights):
+            raise ValueError("MoELayerEP exchanges bf16 rows: it takes MoEWeights, not "
+                             f"{type(local_weights).__name__}")
         self.placement = placement
         self.disp = EPDispatcher(num_experts, group)
         self.peer = None

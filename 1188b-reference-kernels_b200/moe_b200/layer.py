@@ -17,11 +17,11 @@ the per-expert row counts stay on the device.
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Optional
+from typing import Optional, Union
 
 import torch
 
-from . import ops
+from . import fp8, ops
 
 
 @dataclass
@@ -58,21 +58,72 @@ class MoEWeights:
         return MoEWeights(w1, w2)
 
 
-class MoELayer:
-    """Forward of one MoE expert layer on one GPU (inputs already on device)."""
+@dataclass
+class MoEWeightsFp8:
+    """The same weights as e4m3 with one scale for 128 x 128 values: w1 [E,2F,H],
+    w2 [E,H,F] (F a multiple of 128, H of 16). MoELayer then quantises the
+    activations as well, rows with one scale for 128 values."""
+    w1: fp8.Fp8Tensor
+    w2: fp8.Fp8Tensor
 
-    def __init__(self, weights: MoEWeights, topk: int = 8, renorm: bool = True,
-                 expert_bias: Optional[torch.Tensor] = None,
-                 placement: Optional[torch.Tensor] = None):
+    @property
+    def num_experts(self) -> int:
+        return self.w1.data.shape[0]
+
+    @property
+    def hidden(self) -> int:
+        return self.w1.data.shape[2]
+
+    @property
+    def ffn(self) -> int:
+        return self.w2.data.shape[2]
+
+    @staticmethod
+    def from_weights(w: MoEWeights) -> "MoEWeightsFp8":
+        return MoEWeightsFp8(fp8.quantize_fp8_weight(w.w1), fp8.quantize_fp8_weight(w.w2))
+
+
+@dataclass(frozen=True)
+class Routing:
+    """Scores, groups and balance bias of ops.router_group_topk."""
+    score: str = "sigmoid"
+    num_groups: int = 1
+    topk_groups: int = 1
+    group_score: str = "top2"
+    balance_bias: Optional[torch.Tensor] = None
+    scale: float = 1.0
+
+
+class MoELayer:
+    """Forward of one MoE expert layer on one GPU (inputs already on device).
+
+    A layer keeps one group table: run it on one stream at a time. Backward
+    passes of different layers are for one stream at a time as well (two at
+    once, one of them a replayed graph, once met an illegal access whose cause
+    is not known)."""
+
+    def __init__(self, weights: Union[MoEWeights, MoEWeightsFp8], topk: int = 8,
+                 renorm: bool = True, expert_bias: Optional[torch.Tensor] = None,
+                 placement: Optional[torch.Tensor] = None, routing: Optional[Routing] = None):
         """placement (optional int32 [E] permutation): weights[c] is model expert
-        placement[c]; routing, permuted rows and the combine order follow slots."""
+        placement[c]; routing, permuted rows and the combine order follow slots.
+        MoEWeightsFp8: the expert products run in 8 bits, block-scaled.
+        routing: route with ops.router_group_topk instead of the softmax router
+        (no expert_bias, which is added to the logits, and no placement)."""
+        if routing is not None and (expert_bias is not None or placement is not None):
+            raise ValueError("routing takes its bias as balance_bias and no placement")
+        self.fp8 = isinstance(weights, MoEWeightsFp8)
+        if self.fp8 and (weights.ffn % 128 or weights.hidden % 16):
+            raise ValueError(f"8-bit experts need ffn % 128 == 0 and hidden % 16 == 0, got ffn "
+                             f"{weights.ffn} and hidden {weights.hidden}")
+        self.routing = routing
         self.w = weights
         self.k = int(topk)
         self.renorm = renorm
         self.bias = expert_bias
         self.placement = placement
         e = weights.num_experts
-        self.plan = ops.GroupedGemmPlan(e, weights.w1.device)
+        self.plan = ops.GroupedGemmPlan(e, (weights.w1.data if self.fp8 else weights.w1).device)
         self.events = None  # optional dict name -> torch.cuda.Event for stage timing
 
     def _ev(self, name: str):
@@ -104,34 +155,52 @@ class MoELayer:
         self._ev("start")
         # outputs="all": the [T,k] expert list lets the permute read k map
         # entries per token instead of scanning the whole map row
-        if logits is None and self.placement is None and ops.router_gemm_fusable(
-                x, router_weight, self.k):
+        if logits is None and self.placement is None and self.routing is None and \
+                ops.router_gemm_fusable(x, router_weight, self.k):
             r = ops.router_gemm_topk(x, router_weight, self.k, "softmax", self.renorm, self.bias,
-                                     outputs="all")
+                                     outputs="all", return_logits=save_for_backward)
+            if save_for_backward:
+                r, logits = r
         else:
             if logits is None:
                 logits = ops.router_logits(x, router_weight)
-            r = ops.router_topk(logits, self.k, "softmax", self.renorm, self.bias, outputs="all",
-                                placement=self.placement)
+            if self.routing is not None:
+                o = self.routing
+                r = ops.router_group_topk(logits, self.k, o.score, o.num_groups, o.topk_groups,
+                                          o.group_score, o.balance_bias, self.renorm, o.scale)
+            else:
+                r = ops.router_topk(logits, self.k, "softmax", self.renorm, self.bias,
+                                    outputs="all", placement=self.placement)
         rim = ops.row_id_map(r.routing_map, align=1, want_et=False)
         self._ev("routing")
         rows = t * self.k
-        xp, _ = ops.permute(x, rim.map_te, None, num_out=rows, experts=r.topk_idx)
+        if self.fp8:
+            xp = fp8.permute_fp8(x, rim.map_te, r.topk_idx, rows)
+        else:
+            xp, _ = ops.permute(x, rim.map_te, None, num_out=rows, experts=r.topk_idx)
         self._ev("permute")
         self.plan.from_splits(rim.counts, 1)
         y1 = None
-        if save_for_backward:
+        if self.fp8:
+            hmid = fp8.grouped_gemm_fp8(xp, self.w.w1, epilogue="swiglu_fp8", plan=self.plan,
+                                        return_pre=save_for_backward)
+            if save_for_backward:
+                hmid, y1 = hmid
+        elif save_for_backward:
             y1 = ops.grouped_gemm(xp, self.w.w1, plan=self.plan)
             hmid = ops.swiglu(y1)
         else:
             hmid = ops.grouped_gemm(xp, self.w.w1, epilogue="swiglu", plan=self.plan)
         self._ev("fc1")
-        y = ops.grouped_gemm(hmid, self.w.w2, plan=self.plan)
+        if self.fp8:
+            y = fp8.grouped_gemm_fp8(hmid, self.w.w2, plan=self.plan)
+        else:
+            y = ops.grouped_gemm(hmid, self.w.w2, plan=self.plan)
         self._ev("fc2")
         out = ops.unpermute(y, rim.map_te, r.probs, probs_mode="dense", token_major=True)
         self._ev("combine")
         if return_intermediates or save_for_backward:
-            return out, dict(routing=r, rim=rim, xp=xp, y1=y1, h=hmid, y=y)
+            return out, dict(routing=r, rim=rim, xp=xp, y1=y1, h=hmid, y=y, logits=logits)
         return out
 
     __call__ = forward
@@ -147,12 +216,18 @@ class MoELayer:
         combine backward -> fc2 dgrad (dh = dy2 @ W2[e]) and wgrad
         (dW2[e] = dy2^T @ h) -> SwiGLU backward -> fc1 dgrad (dxp = dy1 @
         W1[e]) and wgrad (dW1[e] = dy1^T @ xp) -> permute backward (grad_x[t]
-        = sum over the token's experts of dxp rows). The router's own backward
-        (through softmax, top-k and renormalisation) is the caller's."""
+        = sum over the token's experts of dxp rows). router_backward carries
+        grad_probs on to the logits.
+
+        With 8-bit weights the two dgrads run in 8 bits on quantised dy rows;
+        the wgrads stay in bf16, on dy and on the activations that the forward
+        products took (xp and h as quantised: what dW of those products is)."""
         if ctx.get("y1") is None:
             raise ValueError("ctx must come from forward(..., save_for_backward=True)")
         r, rim = ctx["routing"], ctx["rim"]
-        t, h = ctx["xp"].shape[0] // self.k, ctx["xp"].shape[1]
+        xp, hmid = ctx["xp"], ctx["h"]
+        t, h = (s for s in (xp.data if self.fp8 else xp).shape)
+        t //= self.k
         if grad_out.shape != (t, h):
             raise ValueError(f"grad_out must be [{t},{h}]")
         # The group table of this forward's routing (another forward since may
@@ -160,13 +235,34 @@ class MoELayer:
         # so the backward never waits for the GPU.
         self.plan.from_splits(rim.counts, 1)
         dy2, grad_probs = ops.combine_backward(grad_out, ctx["y"], rim.map_te, r.probs)
-        dh = ops.grouped_gemm(dy2, self.w.w2, plan=self.plan, w_layout="KN")
-        dw2 = ops.grouped_wgrad(dy2, ctx["h"], rim.counts)
+        if self.fp8:
+            dh = fp8.grouped_gemm_fp8(fp8.quantize_fp8(dy2), self.w.w2, plan=self.plan, w_layout="KN")
+            hmid, xp = fp8.dequantize_fp8(hmid), fp8.dequantize_fp8(xp)
+        else:
+            dh = ops.grouped_gemm(dy2, self.w.w2, plan=self.plan, w_layout="KN")
+        dw2 = ops.grouped_wgrad(dy2, hmid, rim.counts)
         dy1 = ops.swiglu_backward(ctx["y1"], dh)
-        dxp = ops.grouped_gemm(dy1, self.w.w1, plan=self.plan, w_layout="KN")
-        dw1 = ops.grouped_wgrad(dy1, ctx["xp"], rim.counts)
+        if self.fp8:
+            dxp = fp8.grouped_gemm_fp8(fp8.quantize_fp8(dy1), self.w.w1, plan=self.plan, w_layout="KN")
+        else:
+            dxp = ops.grouped_gemm(dy1, self.w.w1, plan=self.plan, w_layout="KN")
+        dw1 = ops.grouped_wgrad(dy1, xp, rim.counts)
         grad_x = ops.unpermute(dxp, rim.map_te, None, token_major=True)
         return grad_x, grad_probs, dw1, dw2
+
+    def router_backward(self, grad_probs: torch.Tensor, ctx: dict) -> torch.Tensor:
+        """Gradient of the router logits, [T,E] fp32 (columns: model experts),
+        from the gate gradient that backward returned for the same ctx."""
+        logits, r = ctx.get("logits"), ctx["routing"]
+        if logits is None:
+            raise ValueError("ctx must come from forward(..., save_for_backward=True)")
+        if self.routing is not None:
+            return ops.router_topk_backward(logits, r.topk_idx, grad_probs=grad_probs,
+                                            score=self.routing.score, renorm=self.renorm,
+                                            scale=self.routing.scale)
+        return ops.router_topk_backward(logits, r.topk_idx, grad_probs=grad_probs, score="softmax",
+                                        renorm=self.renorm, bias=self.bias,
+                                        placement=self.placement)
 
 
 def moe_layer_fwd(x: torch.Tensor, logits: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor,
