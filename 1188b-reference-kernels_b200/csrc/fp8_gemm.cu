@@ -142,6 +142,11 @@ MOE_DEVICE void umma_mxf8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uin
 MOE_DEVICE uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
 MOE_DEVICE bool all_lanes(bool v) { return __all_sync(0xffffffffu, v) != 0; }
 
+// Bytes of A that a CTA loads of `rows` rows.
+MOE_DEVICE uint32_t a_bytes(int rows) {
+  return rows <= 0 ? 0u : rows <= kFewRows ? kFewRows * 128u : kTileBytes;
+}
+
 // Tile load into this CTA's shared memory; a pair counts the bytes on the
 // leader's barrier.
 template <bool kPair>
@@ -355,16 +360,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         // pair's CTA loads its own
         const int n0 = p.epilogue == 1 ? tile.n_idx * 128 : tile.n_idx * BN;
         const int n1 = p.epilogue == 1 ? p.f_half + n0 : n0 + 128;
+        // This CTA's A rows: none, few (a box of that height) or a whole box.
+        // The rest of the tile keeps what an earlier one left there: an MMA
+        // row depends on no other.
         const int rows = p.rows[tile.g];
-        // A tile with few rows loads only those (the others keep what an
-        // earlier tile left there: an MMA row depends on no other).
-        const bool few = !kPair && rows - tile.m_idx * kTileM <= kFewRows;
-        const CUtensorMap* map_a = few ? &tmap_a_few : &tmap_a;
-        const uint32_t bytes = kPair ? 2 * kSB : few ? kSB - (128 - kFewRows) * 128u : kSB;
+        const int left = rows - tile.m_idx * kTileM;
+        const int mine = left - static_cast<int>(rank) * 128;
+        const CUtensorMap* map_a = mine <= kFewRows ? &tmap_a_few : &tmap_a;
+        const uint32_t bytes = a_bytes(left) + (kPair ? a_bytes(left - 128) + 2 * kTileBytes : 2 * kTileBytes);
         // A weight that one M-tile reads is not read again: it leaves L2
         // first (32 groups of 100 rows, K 2048: 122 -> 114 us).
-        const uint64_t policy =
-            !kPair && rows <= kTileM ? l2_policy_evict_first() : l2_policy_evict_normal();
+        const uint64_t policy = rows <= kTileM ? l2_policy_evict_first() : l2_policy_evict_normal();
         for (int kb = 0; kb < p.num_kb; ++kb) {
           if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag)) {
             ok = false;
@@ -373,7 +379,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t sa = base + stage * kSB;
           const uint32_t leader_full = O::leader(full_bar(stage));
           if (leader) mbar_arrive_expect_tx(full_bar(stage), bytes);
-          tma_load_3d<kPair>(sa, map_a, kb * 128, row0, 0, leader_full, l2_policy_evict_normal());
+          if (mine > 0)
+            tma_load_3d<kPair>(sa, map_a, kb * 128, row0, 0, leader_full, l2_policy_evict_normal());
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             if (kPair && h != static_cast<int>(rank)) continue;
@@ -741,6 +748,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     else
       tmem_dealloc(tmem, kTmemCols);
   }
+  // Neither SM is given to another kernel's CTA, which allocates TMEM, before
+  // both have released the pair's.
+  if constexpr (kPair) cluster_sync();
 }
 
 // 3-D tensor map over bytes [d2, d1, d0] (d0 contiguous), box 128 x box_rows x 1,
@@ -937,7 +947,7 @@ extern "C" int moe_grouped_gemm_fp8(const void* x, const void* x_scale, const vo
       cfg.attrs = attr;
       cfg.numAttrs = 1;
       MOE_CUDA_CALL(
-          cudaLaunchKernelEx(&cfg, g8::grouped_gemm_fp8_kernel<true>, ta, ta, tb, to, tp, pb),
+          cudaLaunchKernelEx(&cfg, g8::grouped_gemm_fp8_kernel<true>, ta, taf, tb, to, tp, pb),
           "grouped_gemm_fp8 pair launch");
     }
     p.row_start = l.tail_start;

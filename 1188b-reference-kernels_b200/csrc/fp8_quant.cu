@@ -108,13 +108,14 @@ MOE_DEVICE float max8(float a) {  // over the eight lanes of a block
   return a;
 }
 
-constexpr int kRowThreads8 = 128;
+constexpr int kMaxRowThreads = 512;
 constexpr int kMaxTopk = 32;
 
-// One CTA per row (grid-stride over rows). kPermute: the row goes to its
+// One CTA per row (grid-stride over rows), a thread for every unit of it as far
+// as 512 reach, so that a row's loads are all under way at once. kPermute: the row goes to its
 // token's k destinations instead of its own place.
 template <typename U, bool kPermute>
-__global__ void __launch_bounds__(kRowThreads8) quantize_rows_kernel(
+__global__ void __launch_bounds__(kMaxRowThreads) quantize_rows_kernel(
     const typename U::T* __restrict__ x, int64_t rows, int units, int kb, const int64_t* __restrict__ map,
     const int64_t* __restrict__ experts, int k, int64_t E, int64_t num_out,
     uint4* __restrict__ data, uint8_t* __restrict__ scale) {
@@ -130,7 +131,7 @@ __global__ void __launch_bounds__(kRowThreads8) quantize_rows_kernel(
       }
       __syncthreads();
     }
-    for (int u0 = 0; u0 < units; u0 += kRowThreads8) {
+    for (int u0 = 0; u0 < units; u0 += blockDim.x) {
       const int u = u0 + threadIdx.x;
       const bool in = u < units;
       U v;
@@ -248,8 +249,11 @@ int launch_rows(const void* x, int64_t M, int64_t K, const int64_t* map, const i
                 int64_t E, int64_t num_out, void* data, void* scale, cudaStream_t s,
                 const char* who) {
   const int64_t grid = M < (1 << 20) ? M : (1 << 20);
-  quantize_rows_kernel<U, kPermute><<<static_cast<unsigned>(grid), kRowThreads8, 0, s>>>(
-      static_cast<const typename U::T*>(x), M, static_cast<int>(K / kUnit), static_cast<int>((K + kBlock - 1) / kBlock), map, experts,
+  const int units = static_cast<int>(K / kUnit);
+  const int passes = (units + kMaxRowThreads - 1) / kMaxRowThreads;
+  const int threads = (((units + passes - 1) / passes) + 31) / 32 * 32;
+  quantize_rows_kernel<U, kPermute><<<static_cast<unsigned>(grid), threads, 0, s>>>(
+      static_cast<const typename U::T*>(x), M, units, static_cast<int>((K + kBlock - 1) / kBlock), map, experts,
       k, E, num_out, static_cast<uint4*>(data), static_cast<uint8_t*>(scale));
   MOE_CUDA_CHECK_LAUNCH(who);
   return MOE_OK;

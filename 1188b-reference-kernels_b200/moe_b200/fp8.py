@@ -33,9 +33,9 @@ def _blocks(n: int) -> int:
     return -(-n // BLOCK)
 
 
-def _empty(shape, scale_shape, dev) -> Fp8Tensor:
-    return Fp8Tensor(torch.empty(shape, dtype=torch.float8_e4m3fn, device=dev),
-                     torch.empty(scale_shape, dtype=torch.float8_e8m0fnu, device=dev))
+def _empty(like: torch.Tensor, shape, scale_shape) -> Fp8Tensor:
+    return Fp8Tensor(like.new_empty(shape, dtype=torch.float8_e4m3fn),
+                     like.new_empty(scale_shape, dtype=torch.float8_e8m0fnu))
 
 
 def _same_device(**tensors: Optional[torch.Tensor]) -> torch.device:
@@ -82,7 +82,7 @@ def quantize_fp8(x: torch.Tensor) -> Fp8Tensor:
     m, k = x.shape
     _need_k("x", k)
     xc = _aligned(x)
-    out = _empty((m, k), (m, _blocks(k)), dev)
+    out = _empty(xc, (m, k), (m, _blocks(k)))
     with _on(dev):
         _lib.call("moe_quantize_fp8", _p(xc), src, m, k, _p(out.data), _p(out.scale), _stream(dev))
     return out
@@ -98,7 +98,7 @@ def quantize_fp8_weight(w: torch.Tensor) -> Fp8Tensor:
     g, n, k = w.shape
     _need_k("w", k)
     wc = _aligned(w)
-    out = _empty((g, n, k), (g, _blocks(n), _blocks(k)), dev)
+    out = _empty(wc, (g, n, k), (g, _blocks(n), _blocks(k)))
     with _on(dev):
         _lib.call("moe_quantize_fp8_weight", _p(wc), src, g, n, k, _p(out.data), _p(out.scale),
                   _stream(dev))
@@ -114,7 +114,7 @@ def dequantize_fp8(q: Fp8Tensor) -> torch.Tensor:
     _need_fp8("q", q, (m, _blocks(k)))
     _need_k("q.data", k)
     data, scale = _aligned(q.data), q.scale.contiguous()
-    out = torch.empty((m, k), dtype=torch.bfloat16, device=dev)
+    out = data.new_empty((m, k), dtype=torch.bfloat16)
     with _on(dev):
         _lib.call("moe_dequantize_fp8", _p(data), _p(scale), m, k, _p(out), _stream(dev))
     return out
@@ -142,7 +142,7 @@ def permute_fp8(x: torch.Tensor, row_id_map: torch.Tensor, experts: torch.Tensor
     t, h = x.shape
     _need_k("x", h)
     xc, mc, ec = _aligned(x), row_id_map.contiguous(), experts.contiguous()
-    out = _empty((int(num_out), h), (int(num_out), _blocks(h)), dev)
+    out = _empty(xc, (int(num_out), h), (int(num_out), _blocks(h)))
     with _on(dev):
         _lib.call("moe_permute_fp8", _p(xc), _p(mc), _p(ec), ec.shape[1], _p(out.data),
                   _p(out.scale), t, h, mc.shape[1], int(num_out), _stream(dev))
@@ -204,11 +204,11 @@ def grouped_gemm_fp8(x: Fp8Tensor, w: Fp8Tensor,
     xd, xs, wd, ws = _aligned(x.data), x.scale.contiguous(), _aligned(w.data), w.scale.contiguous()
     pre = None
     if epilogue == "none":
-        out, out_scale = torch.empty((rows, n), dtype=torch.bfloat16, device=dev), None
+        out, out_scale = xd.new_empty((rows, n), dtype=torch.bfloat16), None
     else:
-        out, out_scale = _empty((rows, n // 2), (rows, n // 2 // BLOCK), dev)
+        out, out_scale = _empty(xd, (rows, n // 2), (rows, n // 2 // BLOCK))
         if return_pre:
-            pre = torch.empty((rows, n), dtype=torch.bfloat16, device=dev)
+            pre = xd.new_empty((rows, n), dtype=torch.bfloat16)
     with _on(dev):
         _lib.call("moe_grouped_gemm_fp8", _p(xd), _p(xs), _p(wd), _p(ws), _p(out), _p(out_scale),
                   _p(pre), rows, plan.num_groups, g, n, k, 1 if w_layout == "KN" else 0,

@@ -191,10 +191,10 @@ def router_group_topk(logits: torch.Tensor, k: int, score: str = "sigmoid", num_
         bias = bias.contiguous()
     tv = ti = None
     if outputs == "all":
-        tv = torch.empty((t, k), dtype=torch.float32, device=dev)
-        ti = torch.empty((t, k), dtype=torch.int64, device=dev)
-    rmap = torch.empty((t, e), dtype=torch.bool, device=dev)
-    probs = torch.empty((t, e), dtype=torch.float32, device=dev)
+        tv = lg.new_empty((t, k))
+        ti = torch.empty_like(tv, dtype=torch.int64)
+    rmap = torch.empty_like(lg, dtype=torch.bool)
+    probs = torch.empty_like(lg)
     with _on(dev):
         _lib.call("moe_router_group_topk", _p(lg), _p(bias), t, e, int(k),
                   1 if score == "softmax" else 2, int(num_groups), int(topk_groups),
@@ -246,7 +246,7 @@ def router_topk_backward(logits: torch.Tensor, topk_idx: torch.Tensor,
     dev = logits.device
     lg, ix, gv, gp, b, pl = (None if v is None else v.contiguous()
                              for v in (logits, topk_idx, grad_vals, grad_probs, bias, placement))
-    out = torch.empty((t, e), dtype=torch.float32, device=dev)
+    out = torch.empty_like(lg)
     with _on(dev):
         _lib.call("moe_router_topk_backward", _p(lg), _p(b), _p(pl), _p(ix), _p(gv), _p(gp), t, e,
                   k, modes[score], 1 if renorm else 0, float(scale), _p(out), _stream(dev))
