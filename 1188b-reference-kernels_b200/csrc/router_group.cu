@@ -166,7 +166,7 @@ struct RouteArgs {
 // hangs on less than that (0.5 % of the rows of normal logits), or at a NaN;
 // the caller then selects in 64 bits.
 template <int VPL>
-MOE_DEVICE bool select32(const RouteArgs& a, const float* x, int& mine) {
+MOE_DEVICE bool select32(const RouteArgs& a, const float* x, int* s_mine, int& mine) {
   const int lane = lane_id();
   const int size = a.E / a.groups;
   const int g = lane / a.lanes;
@@ -248,39 +248,49 @@ MOE_DEVICE bool select32(const RouteArgs& a, const float* x, int& mine) {
   uint32_t key[VPL];
 #pragma unroll
   for (int j = 0; j < VPL; ++j) key[j] = in && j < n && !odd ? order_key32(c[j]) : 0u;
-  uint32_t best = 0;
+  // A lane offers its best column; its second best stands ready, and only a
+  // lane that wins a third time looks through its columns again.
+  uint32_t b1 = 0, b2 = 0;
+  int c1 = 0, c2 = 0;
 #pragma unroll
-  for (int j = 0; j < VPL; ++j) best = max(best, key[j]);
-  float last = INFINITY;
-  mine = 0;
+  for (int j = 0; j < VPL; ++j) {
+    const bool first = key[j] > b1, second = key[j] > b2;
+    b2 = first ? b1 : second ? key[j] : b2;
+    c2 = first ? c1 : second ? j : c2;
+    b1 = first ? key[j] : b1;
+    c1 = first ? j : c1;
+  }
+  bool spare = true;
+  uint32_t won = 0;                 // lane r: the key of round r
   for (int r = 0; r <= a.k; ++r) {  // one more than is taken: the border below
-    const uint32_t w = __reduce_max_sync(0xffffffffu, best);
-    if (w == 0u) {  // nothing left (all taken, or a NaN: odd)
-      odd |= r < a.k;
-      break;
-    }
-    const float value = key32_value(w);
-    odd |= !(last - value > gap);
-    last = value;
-    if (r == a.k) break;
-    const uint32_t owners = __ballot_sync(0xffffffffu, best == w);
-    const int owner = __ffs(owners) - 1;
-    odd |= (owners & (owners - 1)) != 0u;
-    int col = 0;
+    const uint32_t w = __reduce_max_sync(0xffffffffu, b1);
+    if (lane == r) won = w;
+    if (w == 0u || r == a.k) break;  // nothing left (all taken, or a NaN: odd)
+    const int owner = __ffs(__ballot_sync(0xffffffffu, b1 == w)) - 1;
     if (lane == owner) {
-      best = 0;
+      s_mine[r] = col0 + c1;
+      if (spare) {
+        b1 = b2;
+        c1 = c2;
+        spare = false;
+      } else {
+        b1 = 0;
 #pragma unroll
-      for (int j = 0; j < VPL; ++j) {
-        if (key[j] == w) {
-          key[j] = 0;
-          col = col0 + j;
+        for (int j = 0; j < VPL; ++j) {
+          const bool next = key[j] < w && key[j] > b1;
+          b1 = next ? key[j] : b1;
+          c1 = next ? j : c1;
         }
-        best = max(best, key[j]);
       }
     }
-    col = __shfl_sync(0xffffffffu, col, owner);
-    if (lane == r) mine = col;
   }
+  __syncwarp();
+  mine = lane < a.k ? s_mine[lane] : 0;
+  // Rounds whose keys lie too close (equal ones, of two lanes or of one, come
+  // up in consecutive rounds) leave their order open; so does an empty round.
+  const uint32_t before = __shfl_up_sync(0xffffffffu, won, 1);
+  if (lane < a.k) odd |= won == 0u;
+  if (lane >= 1 && lane <= a.k && won != 0u) odd |= !(key32_value(before) - key32_value(won) > gap);
   return !__any_sync(0xffffffffu, odd);
 }
 
@@ -310,7 +320,8 @@ __global__ void __launch_bounds__(32 * kWarps) router_group_kernel(const RouteAr
   }
   int mine = 0;
   bool done = false;
-  if constexpr (VPL > 0) done = select32<VPL>(a, x, mine);
+  __shared__ int s_mine[kWarps][kMaxK];
+  if constexpr (VPL > 0) done = select32<VPL>(a, x, s_mine[warp_id()], mine);
   Scores64 sc{x, a.bias, 0.0, 1.0, a.softmax != 0, false};
   // The softmax's normaliser cancels in renormalised weights, so that only
   // the 64-bit selection and plain softmax weights need it.
