@@ -10,7 +10,7 @@
 // instruction descriptor selects the byte (k-block index & 3).
 //
 // Two forms of one kernel, persistent, 224 threads a CTA:
-//   pair    clusters of two CTAs (cta_group::2) on 256 x 256 tiles, for groups of at least 256 rows: each CTA
+//   pair    clusters of two CTAs (cta_group::2) on 256 x 256 tiles, for groups of more than 128 rows: each CTA
 //           stages its own 128 A rows and half of the B tile (32 KB a 128-block of K, six stages), the leader
 //           issues M=256, N=256 MMAs over both shared memories into both TMEMs
 //   single  128 x 256 tiles (48 KB a 128-block, four stages) for smaller groups, where the weight stream is
@@ -68,6 +68,11 @@ constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kAccCol1 = 224;  // first column of accumulator 1
 constexpr uint32_t kSfCol = 480;    // TMEM columns of the scales: 4 for A, 8 for B per buffer
 
+// Groups of at most so many rows go to the single form, which keeps more of the
+// weight in flight; above, one pair tile does for two single ones. 32 groups of
+// 100 rows (K 7168, N 4096): 183 us single, 217 pair; 40 of 200 ([K,N], K 4096,
+// N 5120): 253 single, 229 pair.
+constexpr int kSingleRows = 128;
 constexpr int64_t kSlabBytes = 32ll << 20;  // weight bytes walked per pass: they stay in L2 beside the rows
 
 constexpr int kErrProducer = 1;
@@ -93,6 +98,7 @@ struct Params {
   int num_kb;    // 128-blocks along K
   int n_blocks;  // 128-blocks along N
   int n_tiles;
+  int above, most;  // rows of the groups that this launch takes: (above, most]
   int n_chunk;   // pair kernel: N-tiles walked per pass over a group's rows
   int b_mn;      // weight is [num_w, K, N]: B staged MN-major
   int epilogue;  // 0 bf16 out; 1 SwiGLU -> e4m3 rows
@@ -343,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = uniform(*tmem_slot);
   const int groups4 = (p.num_kb + 3) / 4;
 
-  gg::WalkerRT<kTileM> walker{p.rows, p.G, p.n_tiles, 1 << 20, p.n_chunk};
+  gg::WalkerRT<kTileM> walker{p.rows, p.G, p.n_tiles, 1 << 20, p.n_chunk, p.above, p.most};
   Tile tile;
 
   if (warp == 0) {
@@ -914,6 +920,8 @@ extern "C" int moe_grouped_gemm_fp8(const void* x, const void* x_scale, const vo
   p.n_blocks = static_cast<int>((N + 127) / 128);
   p.n_tiles = epilogue == 1 ? p.f_half / 128 : static_cast<int>((N + g8::BN - 1) / g8::BN);
   p.n_chunk = 0;
+  p.above = 0;
+  p.most = 0x7fffffff;
   p.b_mn = w_kn ? 1 : 0;
   p.epilogue = epilogue;
   p.x_words = p.num_kb % 4 == 0 && (reinterpret_cast<uintptr_t>(x_scale) & 3) == 0;
@@ -929,9 +937,11 @@ extern "C" int moe_grouped_gemm_fp8(const void* x, const void* x_scale, const vo
   }
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (clusters > 0) {
-    if (x_rows >= g8::Shape<true>::kTileM) {  // fewer rows: no group has a whole pair tile
+    p.most = g8::kSingleRows;
+    if (x_rows > g8::kSingleRows) {
       g8::Params pb = p;
-      pb.rows = l.rows_body;
+      pb.above = g8::kSingleRows;
+      pb.most = 0x7fffffff;
       pb.n_chunk = static_cast<int>(
           std::min<int64_t>(p.n_tiles, std::max<int64_t>(1, g8::kSlabBytes / (g8::BN * K))));
       cudaLaunchConfig_t cfg = {};
@@ -950,8 +960,6 @@ extern "C" int moe_grouped_gemm_fp8(const void* x, const void* x_scale, const vo
           cudaLaunchKernelEx(&cfg, g8::grouped_gemm_fp8_kernel<true>, ta, taf, tb, to, tp, pb),
           "grouped_gemm_fp8 pair launch");
     }
-    p.row_start = l.tail_start;
-    p.rows = l.rows_tail;
   }
   g8::grouped_gemm_fp8_kernel<false><<<num_sms(dev), g8::kThreads, g8::Shape<false>::kSmemBytes, s>>>(
       ta, taf, tb, to, tp, p);

@@ -66,13 +66,18 @@ struct WalkerRT {
   int n_tiles;
   int raster;
   int n_chunk;
+  int above = 0;            // groups of more than `above` rows ...
+  int most = 0x7fffffff;    // ... and at most `most` are walked
   int g = 0;
   int mt = -1;
   long long base = 0;
 
   __device__ bool locate(long long t, Tile& tile) {
     while (g < G) {
-      if (mt < 0) mt = (max(rows[g], 0) + kTileM - 1) / kTileM;
+      if (mt < 0) {
+        const int r = rows[g];
+        mt = r > above && r <= most ? (r - 1) / kTileM + 1 : 0;
+      }
       const long long cnt = static_cast<long long>(mt) * n_tiles;
       if (t < base + cnt) break;
       base += cnt;
