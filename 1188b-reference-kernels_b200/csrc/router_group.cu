@@ -12,6 +12,14 @@
 // group values formed and compared in 64 bits. A first pass in fp32 with an
 // error bound settles the rows where no decision is that close; the others
 // (one in some hundred) are selected in 64 bits.
+//
+// One warp per token: a row is a kilobyte, its group maxima and its selection
+// are exchanges between lanes, and nothing has to leave the warp. A lane
+// holds consecutive columns of one group, so that a group is a few lanes.
+// Bound by instruction issue (1235 a token): 16384 x 256, 8 groups of which 4
+// stay, top-8: 34 us on the device against 6.0 us of bytes; 4 tokens: 5.0 us.
+// The gradient reads what a row needs and writes it once: 16384 x 256 from a
+// sigmoid 10 us (2.9 us of bytes).
 #include <math.h>
 
 #include "moe_common.cuh"

@@ -314,3 +314,42 @@ def test_gemm_uniform_splits_streams_and_graph(cuda_dev):
         counts.copy_(torch.tensor(c, dtype=torch.int32))
         graph.replay()
         assert torch.equal(out, moe_b200.grouped_gemm_fp8(moe_b200.quantize_fp8(xin), w, c))
+
+
+def test_gemm_groups_that_share_weights(cuda_dev):
+    """The group table of expert-parallel receive buffers: rows of one expert from several sources."""
+    import moe_b200
+    src, nw = 3, 4
+    x, w = _operands(cuda_dev, 700, nw, 256, 384, "NK", 21)
+    counts = [[10, 0, 200, 40], [150, 1, 129, 20], [0, 60, 50, 40]]
+    plan = moe_b200.GroupedGemmPlan(src * nw, cuda_dev).from_ep_counts(
+        torch.tensor(counts).flatten(), src, nw)
+    got = moe_b200.grouped_gemm_fp8(x, w, plan=plan).double()
+    assert plan.device_error() == 0
+    at = 0
+    for s in range(src):  # source-major rows
+        y, m = _product64(moe_b200.Fp8Tensor(x.data[at:at + sum(counts[s])], x.scale[at:at + sum(counts[s])]),
+                          w, counts[s], "NK")
+        d = (got[at:at + sum(counts[s])] - y).abs()
+        assert bool((d <= 2.0 ** -8 * y.abs() + 1.01 * 384 * 2.0 ** -24 * m).all())
+        at += sum(counts[s])
+
+
+def test_offsets_past_32_bits(cuda_dev):
+    """Outputs and inputs of more than 2^31 elements: the last rows are as those of a small call."""
+    import moe_b200
+    rows, n, k = 270000, 8192, 128
+    x, w = _operands(cuda_dev, 4096, 2, n, k, "NK", 31)
+    big = moe_b200.Fp8Tensor(x.data.repeat(66, 1)[:rows],
+                             ref.bytes_of(x.scale).repeat(66, 1)[:rows].view(torch.float8_e8m0fnu))
+    y = moe_b200.grouped_gemm_fp8(big, w, [100, rows - 100])
+    tail = moe_b200.Fp8Tensor(big.data[-300:], big.scale[-300:])
+    assert torch.equal(y[-300:], moe_b200.grouped_gemm_fp8(tail, w, [0, 300]))
+    del y, big
+    a = torch.randn(2048, 16384, device=cuda_dev).to(torch.bfloat16)
+    q = moe_b200.quantize_fp8(a)
+    qq = moe_b200.quantize_fp8(a.repeat(66, 1))
+    assert torch.equal(ref.bytes_of(qq.data[-2048:]), ref.bytes_of(q.data))
+    assert torch.equal(ref.bytes_of(qq.scale[-2048:]), ref.bytes_of(q.scale))
+    back = moe_b200.dequantize_fp8(qq)
+    assert torch.equal(back[-2048:], moe_b200.dequantize_fp8(q))
