@@ -9,12 +9,17 @@
 // 32-bit cell per row holding the bytes of four consecutive 128-blocks; the
 // instruction descriptor selects the byte (k-block index & 3).
 //
-// Two forms of one kernel, persistent, 224 threads a CTA:
+// Three forms of one kernel, persistent, 224 threads a CTA:
 //   pair    clusters of two CTAs (cta_group::2) on 256 x 256 tiles, for groups of more than 128 rows: each CTA
 //           stages its own 128 A rows and half of the B tile (32 KB a 128-block of K, six stages), the leader
 //           issues M=256, N=256 MMAs over both shared memories into both TMEMs
 //   single  128 x 256 tiles (48 KB a 128-block, four stages) for smaller groups, where the weight stream is
 //           what takes the time
+//   few     the same for calls of at most 32 rows in all: A tiles of 32 rows, so that six stages fit and half as
+//           much weight again is on its way (K 7168, N 4096, 32 rows over 20 groups: 133 -> 119 us; one row: 38 ->
+//           32 us). The MMAs read 128 rows from the A tile's place all the same; what lies behind it only enters
+//           rows that nobody stores. As a launch of its own beside the single form it gave nothing (512 rows over
+//           32 groups 181 against 183 us, 768 rows of which half in larger groups 193 against 183)
 // Warps:
 //   warp 0     TMA producer
 //   warp 1     TMEM owner; copies scales to TMEM (tcgen05.cp) and issues the MMAs (K=32)
@@ -28,8 +33,8 @@
 // the rest of a tile's epilogue overlaps the next tile's mainloop.
 // Measured (one B200 at its 1000 W, 1.2 to 1.5 GHz): 32 groups of 1024 rows,
 // K 7168, N 4096 with SwiGLU 0.89-0.93 ms, K 2048, N 7168 0.50-0.52 ms (2070
-// and 1860 TFLOP/s; power bounds both); 20 groups of one or two rows 122 us,
-// 4.8 TB/s of weights.
+// and 1860 TFLOP/s; power bounds both); 20 groups of one or two rows 119 us,
+// 4.9 TB/s of weights.
 // Rows are described by the group table of moe_grouped_gemm_plan_*. Every
 // wait is bounded (2 s): on timeout the kernel records an error word, drains
 // its copies and MMAs, frees TMEM and returns.
@@ -51,20 +56,24 @@ using gg::wait_drain;
 constexpr int BN = 256;
 constexpr int kThreads = 224;
 constexpr uint32_t kTileBytes = 128 * 128;  // 128 rows (or reduction rows) x 128 bytes
-constexpr int kFewRows = 32;   // single CTA: M-tiles of at most so many rows load a box of that height
+constexpr int kFewRows = 32;   // rows of the small A box, and of a call of the few form
 constexpr int kSfStages = 6;   // scale buffers in shared memory
 constexpr int kSfTmem = 2;     // and in TMEM
 constexpr int kSfBatch = 4;    // K groups whose scales are loaded at once
 constexpr uint32_t kSfBytes = 512 + 1024;    // 128 A rows and 256 B rows, one 32-bit cell each
 constexpr uint32_t kEpiWarpBytes = 4096;     // per epilogue warp: two 32 x 64-byte boxes or one 32 x 128-byte box
 
-template <bool kPair>
+enum Form { kPairForm, kSingleForm, kFewForm };
+
+template <Form kForm>
 struct Shape {
-  static constexpr int kTileM = kPair ? 256 : 128;
-  static constexpr int kStages = kPair ? 6 : 4;
-  static constexpr uint32_t kStageBytes = (kPair ? 2 : 3) * kTileBytes;  // of one CTA: A, half of B or all
+  static constexpr int kTileM = kForm == kPairForm ? 256 : 128;
+  static constexpr int kStages = kForm == kSingleForm ? 4 : 6;
+  static constexpr uint32_t kABytes = kForm == kFewForm ? kFewRows * 128u : kTileBytes;
+  static constexpr uint32_t kStageBytes = kABytes + (kForm == kPairForm ? 1 : 2) * kTileBytes;  // of one CTA
+  static constexpr uint32_t kEpiBytes = kForm == kFewForm ? 0u : 4 * kEpiWarpBytes;
   static constexpr size_t kSmemBytes =
-      1024 + kStages * kStageBytes + 4 * kEpiWarpBytes + kSfStages * kSfBytes + 512;
+      1024 + kStages * kStageBytes + kEpiBytes + kSfStages * kSfBytes + 512;
   static_assert(kSmemBytes <= 232448, "shared memory per CTA");
 };
 
@@ -276,24 +285,27 @@ struct Op {
   }
 };
 
-template <bool kPair>
+template <Form kForm>
 __global__ void __launch_bounds__(kThreads, 1)
     grouped_gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_a,
                             const __grid_constant__ CUtensorMap tmap_a_few,
                             const __grid_constant__ CUtensorMap tmap_b,
                             const __grid_constant__ CUtensorMap tmap_out,
                             const __grid_constant__ CUtensorMap tmap_pre, const Params p) {
+  constexpr bool kPair = kForm == kPairForm;
+  constexpr bool kFew = kForm == kFewForm;
   using O = Op<kPair>;
-  constexpr int kTileM = Shape<kPair>::kTileM;
-  constexpr int kS = Shape<kPair>::kStages;
-  constexpr uint32_t kSB = Shape<kPair>::kStageBytes;
+  constexpr int kTileM = Shape<kForm>::kTileM;
+  constexpr int kS = Shape<kForm>::kStages;
+  constexpr uint32_t kSB = Shape<kForm>::kStageBytes;
+  constexpr uint32_t kAB = Shape<kForm>::kABytes;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t base = (raw_addr + 1023u) & ~1023u;
   uint8_t* base_ptr = smem_raw + (base - raw_addr);
   const uint32_t epi_base = base + kS * kSB;
-  const uint32_t sf_base = epi_base + 4 * kEpiWarpBytes;
-  uint8_t* sf_ptr = base_ptr + kS * kSB + 4 * kEpiWarpBytes;
+  const uint32_t sf_base = epi_base + Shape<kForm>::kEpiBytes;
+  uint8_t* sf_ptr = base_ptr + kS * kSB + Shape<kForm>::kEpiBytes;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sf_ptr + kSfStages * kSfBytes);
   const uint32_t bar0 = smem_u32(bars);
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
@@ -376,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int rows = p.rows[tile.g];
         const int left = rows - tile.m_idx * kTileM;
         const int mine = left - static_cast<int>(rank) * 128;
-        const CUtensorMap* map_a = mine <= kFewRows ? &tmap_a_few : &tmap_a;
+        const CUtensorMap* map_a = kFew || mine <= kFewRows ? &tmap_a_few : &tmap_a;
         const uint32_t bytes = a_bytes(left) + (kPair ? a_bytes(left - 128) + 2 * kTileBytes : 2 * kTileBytes);
         // A weight that one M-tile reads is not read again: it leaves L2
         // first (32 groups of 100 rows, K 2048: 122 -> 114 us).
@@ -395,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int h = 0; h < 2; ++h) {
             if (kPair && h != static_cast<int>(rank)) continue;
             const int n = h ? n1 : n0;
-            tma_load_3d<kPair>(sa + (kPair ? 1 : 1 + h) * kTileBytes, &tmap_b, p.b_mn ? n : kb * 128,
+            tma_load_3d<kPair>(sa + kAB + (kPair ? 0 : h) * kTileBytes, &tmap_b, p.b_mn ? n : kb * 128,
                                p.b_mn ? kb * 128 : n, wi, leader_full, policy);
           }
           ++issued;
@@ -496,8 +508,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_fence_after();
             const uint32_t sa = base + stage * kSB;
             const uint64_t ad = umma_desc_k_sw128(sa);
-            const uint64_t bd = p.b_mn ? umma_desc_mn_sw128(sa + kTileBytes, kTileBytes)
-                                       : umma_desc_k_sw128(sa + kTileBytes);
+            const uint64_t bd = p.b_mn ? umma_desc_mn_sw128(sa + kAB, kTileBytes)
+                                       : umma_desc_k_sw128(sa + kAB);
             const uint32_t id = with_sf_id(idesc, static_cast<uint32_t>(i));
             if (issuer) {
 #pragma unroll
@@ -601,7 +613,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t row = static_cast<int64_t>(p.row_start[tile.g]) + m_local;
       const bool rvalid = m_local < p.rows[tile.g] && row < p.x_rows;
       // a warp whose 32 rows all belong to the group stores them with TMA
-      const bool tma = __all_sync(0xffffffffu, rvalid);
+      const bool tma = !kFew && __all_sync(0xffffffffu, rvalid);
       const int warp_row0 = static_cast<int>(row) - lane;
       const uint32_t tbase =
           tmem + (static_cast<uint32_t>(quad * 32) << 16) + (acc ? kAccCol1 : 0u);
@@ -818,18 +830,22 @@ int prepare_device(int dev, int* clusters) {
     *clusters = pairs[dev];
     return MOE_OK;
   }
-  MOE_CUDA_CALL(cudaFuncSetAttribute(grouped_gemm_fp8_kernel<false>,
+  MOE_CUDA_CALL(cudaFuncSetAttribute(grouped_gemm_fp8_kernel<kPairForm>,
                                      cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     static_cast<int>(Shape<false>::kSmemBytes)),
-                "cudaFuncSetAttribute(grouped_gemm_fp8)");
-  MOE_CUDA_CALL(cudaFuncSetAttribute(grouped_gemm_fp8_kernel<true>,
+                                     static_cast<int>(Shape<kPairForm>::kSmemBytes)),
+                "cudaFuncSetAttribute(grouped_gemm_fp8 pair)");
+  MOE_CUDA_CALL(cudaFuncSetAttribute(grouped_gemm_fp8_kernel<kSingleForm>,
                                      cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     static_cast<int>(Shape<true>::kSmemBytes)),
-                "cudaFuncSetAttribute(grouped_gemm_fp8_pair)");
+                                     static_cast<int>(Shape<kSingleForm>::kSmemBytes)),
+                "cudaFuncSetAttribute(grouped_gemm_fp8 single)");
+  MOE_CUDA_CALL(cudaFuncSetAttribute(grouped_gemm_fp8_kernel<kFewForm>,
+                                     cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     static_cast<int>(Shape<kFewForm>::kSmemBytes)),
+                "cudaFuncSetAttribute(grouped_gemm_fp8 few)");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * 74);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Shape<true>::kSmemBytes;
+  cfg.dynamicSmemBytes = Shape<kPairForm>::kSmemBytes;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
@@ -838,7 +854,7 @@ int prepare_device(int dev, int* clusters) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   int n = 0;
-  if (cudaOccupancyMaxActiveClusters(&n, grouped_gemm_fp8_kernel<true>, &cfg) != cudaSuccess) n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, grouped_gemm_fp8_kernel<kPairForm>, &cfg) != cudaSuccess) n = 0;
   cudaGetLastError();  // clear a non-sticky error of the query
   if (dev >= 0 && dev < 64) {
     pairs[dev] = n;
@@ -951,7 +967,7 @@ extern "C" int moe_grouped_gemm_fp8(const void* x, const void* x_scale, const vo
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3(2 * clusters);
       cfg.blockDim = dim3(g8::kThreads);
-      cfg.dynamicSmemBytes = g8::Shape<true>::kSmemBytes;
+      cfg.dynamicSmemBytes = g8::Shape<g8::kPairForm>::kSmemBytes;
       cfg.stream = s;
       cudaLaunchAttribute attr[1];
       attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -961,12 +977,18 @@ extern "C" int moe_grouped_gemm_fp8(const void* x, const void* x_scale, const vo
       cfg.attrs = attr;
       cfg.numAttrs = 1;
       MOE_CUDA_CALL(
-          cudaLaunchKernelEx(&cfg, g8::grouped_gemm_fp8_kernel<true>, ta, taf, tb, to, tp, pb),
+          cudaLaunchKernelEx(&cfg, g8::grouped_gemm_fp8_kernel<g8::kPairForm>, ta, taf, tb, to, tp, pb),
           "grouped_gemm_fp8 pair launch");
     }
   }
-  g8::grouped_gemm_fp8_kernel<false><<<num_sms(dev), g8::kThreads, g8::Shape<false>::kSmemBytes, s>>>(
-      ta, taf, tb, to, tp, p);
+  if (x_rows <= g8::kFewRows) {
+    g8::grouped_gemm_fp8_kernel<g8::kFewForm>
+        <<<num_sms(dev), g8::kThreads, g8::Shape<g8::kFewForm>::kSmemBytes, s>>>(ta, taf, tb, to, tp, p);
+    MOE_CUDA_CHECK_LAUNCH("grouped_gemm_fp8 few launch");
+    return MOE_OK;
+  }
+  g8::grouped_gemm_fp8_kernel<g8::kSingleForm>
+      <<<num_sms(dev), g8::kThreads, g8::Shape<g8::kSingleForm>::kSmemBytes, s>>>(ta, taf, tb, to, tp, p);
   MOE_CUDA_CHECK_LAUNCH("grouped_gemm_fp8 launch");
   return MOE_OK;
 }
