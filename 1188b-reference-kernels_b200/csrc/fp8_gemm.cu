@@ -246,6 +246,10 @@ struct Op {
     if constexpr (kPair) return mbar_wait_cluster(bar, parity, abort_flag);
     return mbar_wait(bar, parity, abort_flag);
   }
+  static MOE_DEVICE bool try_wait(uint32_t bar, uint32_t parity) {
+    if constexpr (kPair) return mbar_try_wait_cluster(bar, parity);
+    return mbar_try_wait(bar, parity);
+  }
   // a commit that both CTAs see / that the issuing CTA alone needs
   static MOE_DEVICE void commit(uint32_t bar) {
     if constexpr (kPair)
@@ -452,9 +456,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       // Scales of the next K group (the pair's groups in order, across tiles) to the
       // TMEM buffer that the group before the current one has used. Called in
       // the middle of a group, so that neither wait is for work just issued.
-      auto copy_scales = [&]() {
+      auto scales_ready = [&]() {  // without waiting
+        return all_lanes(mbar_try_wait(sf_used(copied & 1), static_cast<uint32_t>((copied >> 1) & 1) ^ 1u) &&
+                         O::try_wait(sf_full(sf), sf_phase));
+      };
+      auto copy_scales = [&](bool are_ready) {
         const uint32_t b = static_cast<uint32_t>(copied & 1);
-        if (!all_lanes(mbar_wait(sf_used(b), static_cast<uint32_t>((copied >> 1) & 1) ^ 1u, abort_flag) &&
+        if (!are_ready &&
+            !all_lanes(mbar_wait(sf_used(b), static_cast<uint32_t>((copied >> 1) & 1) ^ 1u, abort_flag) &&
                        O::wait(sf_full(sf), sf_phase, abort_flag)))
           return false;
         tc_fence_after();
@@ -477,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       long long t = cid;
       bool more = all_lanes(walker.locate(t, tile));
-      if (more) ok = copy_scales();
+      if (more) ok = copy_scales(false);
       while (ok && more) {
         t += ncl;
         more = all_lanes(walker.locate(t, tile));  // whether another tile follows
@@ -504,6 +513,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             // so that the answer's latency does not stand between the two
             const int next = stage + 1 == kS ? 0 : stage + 1;
             ready = all_lanes(mbar_try_wait(full_bar(next), next == 0 ? phase ^ 1u : phase));
+            const bool copy = i == min(2, n - 1) && (kg + 1 < groups4 || more);
+            const bool sf_ready = copy && scales_ready();
             tc_fence_after();
             const uint32_t sa = base + stage * kSB;
             const uint64_t ad = umma_desc_k_sw128(sa);
@@ -522,7 +533,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               stage = 0;
               phase ^= 1u;
             }
-            if (i == min(1, n - 1) && (kg + 1 < groups4 || more) && !copy_scales()) {
+            if (copy && !copy_scales(sf_ready)) {
               ok = false;
               break;
             }
