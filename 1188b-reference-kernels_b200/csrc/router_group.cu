@@ -16,8 +16,10 @@
 // One warp per token: a row is a kilobyte, its group maxima and its selection
 // are exchanges between lanes, and nothing has to leave the warp. A lane
 // holds consecutive columns of one group, so that a group is a few lanes.
-// Bound by instruction issue (1235 a token): 16384 x 256, 8 groups of which 4
-// stay, top-8: 34 us on the device against 6.0 us of bytes; 4 tokens: 5.0 us.
+// Bound by instruction issue, about a thousand a token, and at the end by the
+// latency of a row that needs 64 bits (selected by a copy of c in shared
+// memory that took 10 us of 34): 16384 x 256, 8 groups of which 4 stay, top-8:
+// 29 us on the device against 6.0 us of bytes; 4 tokens: 4.8 us.
 // The gradient reads what a row needs and writes it once: 16384 x 256 from a
 // sigmoid 10 us (2.9 us of bytes).
 #include <math.h>
@@ -302,8 +304,84 @@ MOE_DEVICE bool select32(const RouteArgs& a, const float* x, int* s_mine, int& m
   return !__any_sync(0xffffffffu, odd);
 }
 
-// One warp per token. VPL 0: 64 bits throughout (shapes whose lanes would
-// hold more than 16 columns).
+// The larger of two 64-bit keys over the warp, as two 32-bit maxima; `owners`
+// gets the lanes that hold it.
+MOE_DEVICE uint64_t warp_max_key(uint64_t key, uint32_t& owners) {
+  const uint32_t hi = static_cast<uint32_t>(key >> 32), lo = static_cast<uint32_t>(key);
+  const uint32_t mhi = __reduce_max_sync(0xffffffffu, hi);
+  const uint32_t mlo = __reduce_max_sync(0xffffffffu, hi == mhi ? lo : 0u);
+  owners = __ballot_sync(0xffffffffu, hi == mhi && lo == mlo);
+  return static_cast<uint64_t>(mhi) << 32 | mlo;
+}
+
+// Selection in 64 bits in the lane layout of select32 (columns rise with the
+// lane, so the lowest owner of a key has the lowest column).
+template <int VPL>
+MOE_DEVICE int select64_lanes(const RouteArgs& a, const Scores64& sc, int* s_mine) {
+  const int lane = lane_id();
+  const int size = a.E / a.groups;
+  const int g = lane / a.lanes;
+  const int first = (lane & (a.lanes - 1)) * a.vpl;
+  const int n = g < a.groups ? max(0, min(a.vpl, size - first)) : 0;
+  const int col0 = g * size + first;
+  uint64_t key[VPL];
+  double hi = -INFINITY, lo = -INFINITY;
+  bool nan = false;
+#pragma unroll
+  for (int j = 0; j < VPL; ++j) {
+    key[j] = 0;
+    if (j < n) {
+      const double c = sc.c(col0 + j);
+      nan |= isnan(c);
+      lo = fmax(lo, fmin(hi, c));
+      hi = fmax(hi, c);
+      key[j] = order_key(c);
+    }
+  }
+  if (a.keep < a.groups) {
+    for (int off = 1; off < a.lanes; off <<= 1) {
+      const double h2 = __shfl_xor_sync(0xffffffffu, hi, off);
+      const double l2 = __shfl_xor_sync(0xffffffffu, lo, off);
+      nan |= __shfl_xor_sync(0xffffffffu, static_cast<int>(nan), off) != 0;
+      lo = fmax(fmin(hi, h2), fmax(lo, l2));
+      hi = fmax(hi, h2);
+    }
+    // a NaN counts as the largest value of its group
+    const uint64_t rank = nan ? ~0ull : order_key(a.top2 && size > 1 ? hi + lo : hi);
+    int better = 0;
+    for (int q = 0; q < a.groups; ++q) {
+      const uint64_t other = __shfl_sync(0xffffffffu, rank, q * a.lanes);
+      better += other > rank || (other == rank && q < g);
+    }
+    if (better >= a.keep) {
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) key[j] = 0;
+    }
+  }
+  for (int r = 0; r < a.k; ++r) {
+    uint64_t best = 0;
+    int at = 0;
+#pragma unroll
+    for (int j = 0; j < VPL; ++j)
+      if (key[j] > best) {
+        best = key[j];
+        at = j;
+      }
+    uint32_t owners;
+    warp_max_key(best, owners);
+    if (lane == __ffs(owners) - 1) {
+      s_mine[r] = col0 + at;
+#pragma unroll
+      for (int j = 0; j < VPL; ++j)
+        if (j == at) key[j] = 0;
+    }
+  }
+  __syncwarp();
+  return lane < a.k ? s_mine[lane] : 0;
+}
+
+// One warp per token. VPL 0: 64 bits throughout, the scores in shared memory
+// (shapes whose lanes would hold more than 16 columns).
 template <int VPL>
 __global__ void __launch_bounds__(32 * kWarps) router_group_kernel(const RouteArgs a) {
   extern __shared__ double s_c[];
@@ -340,7 +418,12 @@ __global__ void __launch_bounds__(32 * kWarps) router_group_kernel(const RouteAr
     sc.none = sc.m == -INFINITY;
     if (!done || !a.renorm) sc.z = softmax_sum64(x, a.E, sc.m);
   }
-  if (!done) mine = select64(sc, s_c + warp_id() * a.E, a.E, a.k, a.groups, a.keep, a.top2);
+  if (!done) {
+    if constexpr (VPL > 0)
+      mine = select64_lanes<VPL>(a, sc, s_mine[warp_id()]);
+    else
+      mine = select64(sc, s_c + warp_id() * a.E, a.E, a.k, a.groups, a.keep, a.top2);
+  }
   double weight = lane < a.k ? sc.s(mine) : 0.0;
   if (a.renorm) {
     const double sum = warp_sum(weight);
@@ -359,7 +442,7 @@ __global__ void __launch_bounds__(32 * kWarps) router_group_kernel(const RouteAr
 template <int VPL>
 void launch_route(const RouteArgs& a, cudaStream_t s) {
   router_group_kernel<VPL><<<static_cast<unsigned>((a.T + kWarps - 1) / kWarps), 32 * kWarps,
-                             kWarps * a.E * sizeof(double), s>>>(a);
+                             VPL > 0 ? 0 : kWarps * a.E * sizeof(double), s>>>(a);
 }
 
 // One warp per token; lane j < k holds the j-th selected expert.
