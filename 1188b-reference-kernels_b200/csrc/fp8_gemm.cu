@@ -185,13 +185,13 @@ MOE_DEVICE void tma_load_3d(uint32_t dst, const void* tmap, int32_t x, int32_t y
 }
 
 // Four scale bytes kb0..kb0+3 of a row of `num_kb` bytes at p (1.0 past its
-// end), `step` bytes apart; one load where every such row starts on a word.
-MOE_DEVICE uint32_t scale_cell(const uint8_t* p, int64_t step, int kb0, int num_kb, bool words) {
+// end); one load where every such row starts on a word.
+MOE_DEVICE uint32_t scale_cell(const uint8_t* p, int kb0, int num_kb, bool words) {
   if (words) return __ldg(reinterpret_cast<const uint32_t*>(p + kb0));
   uint32_t w = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t b = kb0 + i < num_kb ? __ldg(p + (kb0 + i) * step) : fp8::kOne;
+    const uint32_t b = kb0 + i < num_kb ? __ldg(p + kb0 + i) : fp8::kOne;
     w |= b << (8 * i);
   }
   return w;
@@ -204,15 +204,26 @@ MOE_DEVICE void load_scale_cells(const Params& p, int64_t row0, int64_t wi, int 
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     const int64_t r = row0 + c * 32 + lane;
-    a[c] = r < p.x_rows ? scale_cell(p.xs + r * p.num_kb, 1, kg * 4, p.num_kb, p.x_words) : 0x7F7F7F7Fu;
+    a[c] = r < p.x_rows ? scale_cell(p.xs + r * p.num_kb, kg * 4, p.num_kb, p.x_words) : 0x7F7F7F7Fu;
+  }
+  if (p.b_mn) {  // bytes of one block lie a row of blocks apart: a lane loads each
+    const int nb = lane & 4 ? nb1 : nb0;
+    const int kb = kg * 4 + (lane & 3);
+    uint32_t v = fp8::kOne;
+    if (lane < 8 && nb < p.n_blocks && wi < p.num_w && kb < p.num_kb)
+      v = __ldg(p.ws + (wi * p.num_kb + kb) * p.n_blocks + nb);
+    v <<= 8 * (lane & 3);
+    v |= __shfl_xor_sync(0xffffffffu, v, 1);
+    v |= __shfl_xor_sync(0xffffffffu, v, 2);
+    b[0] = __shfl_sync(0xffffffffu, v, 0);
+    b[1] = __shfl_sync(0xffffffffu, v, 4);
+    return;
   }
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int nb = h ? nb1 : nb0;
-    const int64_t w0 =
-        p.b_mn ? wi * p.num_kb * p.n_blocks + nb : (wi * p.n_blocks + nb) * p.num_kb;
     b[h] = nb < p.n_blocks && wi < p.num_w
-               ? scale_cell(p.ws + w0, p.b_mn ? p.n_blocks : 1, kg * 4, p.num_kb, p.w_words)
+               ? scale_cell(p.ws + (wi * p.n_blocks + nb) * p.num_kb, kg * 4, p.num_kb, p.w_words)
                : 0x7F7F7F7Fu;
   }
 }
