@@ -92,13 +92,23 @@ constexpr int kErrMma = 2;
 constexpr int kErrEpilogue = 3;
 constexpr int kErrScales = 5;
 
+// Scale bytes at 4 kg .. 4 kg + 3 of row `row` of a [rows, num_kb] byte matrix
+// of `total` bytes, 1.0 past the row's end. Rows that are whole words take one
+// load, other rows of a word-aligned matrix two neighbouring words.
+struct ScaleRows {
+  const uint8_t* p;
+  int64_t total;
+  int num_kb;
+  bool aligned;  // p is a multiple of 4
+};
+
 struct Params {
   const int32_t* row_start;
   const int32_t* rows;
   const int32_t* widx;
   int32_t* err;
-  const uint8_t* xs;   // [x_rows, num_kb]
-  const uint8_t* ws;   // NK: [num_w, n_blocks, num_kb]; KN: [num_w, num_kb, n_blocks]
+  ScaleRows xs;        // [x_rows, num_kb]
+  ScaleRows ws;        // NK: [num_w, n_blocks, num_kb]; KN: [num_w, num_kb, n_blocks] (by bytes)
   void* out;           // bf16 [x_rows, N], or e4m3 [x_rows, F]
   uint8_t* out_scale;  // [x_rows, F / 128] (epilogue 1)
   __nv_bfloat16* pre;  // bf16 [x_rows, N] gate|up (epilogue 1, nullable)
@@ -114,7 +124,6 @@ struct Params {
   int n_chunk;   // pair kernel: N-tiles walked per pass over a group's rows
   int b_mn;      // weight is [num_w, K, N]: B staged MN-major
   int epilogue;  // 0 bf16 out; 1 SwiGLU -> e4m3 rows
-  bool x_words, w_words;  // scale rows are whole 32-bit words
 };
 
 // Instruction descriptor, kind::mxf8f6f4: D fp32, A and B e4m3, E8M0 scales;
@@ -184,15 +193,22 @@ MOE_DEVICE void tma_load_3d(uint32_t dst, const void* tmap, int32_t x, int32_t y
         : "memory");
 }
 
-// Four scale bytes kb0..kb0+3 of a row of `num_kb` bytes at p (1.0 past its
-// end); one load where every such row starts on a word.
-MOE_DEVICE uint32_t scale_cell(const uint8_t* p, int kb0, int num_kb, bool words) {
-  if (words) return __ldg(reinterpret_cast<const uint32_t*>(p + kb0));
+MOE_DEVICE uint32_t scale_cell(const ScaleRows& m, int64_t row, int kg) {
+  const int64_t at = row * m.num_kb + kg * 4;
+  const uint32_t* words = reinterpret_cast<const uint32_t*>(m.p) + (at >> 2);
+  if (m.aligned && m.num_kb % 4 == 0) return __ldg(words);
   uint32_t w = 0;
+  if (m.aligned && (at & ~3ll) + 8 <= m.total) {
+    w = __funnelshift_r(__ldg(words), __ldg(words + 1), static_cast<uint32_t>(at & 3) * 8u);
+  } else {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t b = kb0 + i < num_kb ? __ldg(p + kb0 + i) : fp8::kOne;
-    w |= b << (8 * i);
+    for (int i = 0; i < 4; ++i)
+      if (at + i < m.total) w |= static_cast<uint32_t>(__ldg(m.p + at + i)) << (8 * i);
+  }
+  const int live = m.num_kb - kg * 4;  // bytes before the row's end
+  if (live < 4) {
+    const uint32_t mask = (1u << (8 * live)) - 1u;
+    w = (w & mask) | (0x7F7F7F7Fu & ~mask);
   }
   return w;
 }
@@ -204,14 +220,14 @@ MOE_DEVICE void load_scale_cells(const Params& p, int64_t row0, int64_t wi, int 
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     const int64_t r = row0 + c * 32 + lane;
-    a[c] = r < p.x_rows ? scale_cell(p.xs + r * p.num_kb, kg * 4, p.num_kb, p.x_words) : 0x7F7F7F7Fu;
+    a[c] = r < p.x_rows ? scale_cell(p.xs, r, kg) : 0x7F7F7F7Fu;
   }
   if (p.b_mn) {  // bytes of one block lie a row of blocks apart: a lane loads each
     const int nb = lane & 4 ? nb1 : nb0;
     const int kb = kg * 4 + (lane & 3);
     uint32_t v = fp8::kOne;
     if (lane < 8 && nb < p.n_blocks && wi < p.num_w && kb < p.num_kb)
-      v = __ldg(p.ws + (wi * p.num_kb + kb) * p.n_blocks + nb);
+      v = __ldg(p.ws.p + (wi * p.num_kb + kb) * p.n_blocks + nb);
     v <<= 8 * (lane & 3);
     v |= __shfl_xor_sync(0xffffffffu, v, 1);
     v |= __shfl_xor_sync(0xffffffffu, v, 2);
@@ -223,7 +239,7 @@ MOE_DEVICE void load_scale_cells(const Params& p, int64_t row0, int64_t wi, int 
   for (int h = 0; h < 2; ++h) {
     const int nb = h ? nb1 : nb0;
     b[h] = nb < p.n_blocks && wi < p.num_w
-               ? scale_cell(p.ws + (wi * p.n_blocks + nb) * p.num_kb, kg * 4, p.num_kb, p.w_words)
+               ? scale_cell(p.ws, wi * p.n_blocks + nb, kg)
                : 0x7F7F7F7Fu;
   }
 }
@@ -943,8 +959,6 @@ extern "C" int moe_grouped_gemm_fp8(const void* x, const void* x_scale, const vo
   p.rows = l.rows;
   p.widx = l.widx;
   p.err = l.err;
-  p.xs = static_cast<const uint8_t*>(x_scale);
-  p.ws = static_cast<const uint8_t*>(w_scale);
   p.out = out;
   p.out_scale = static_cast<uint8_t*>(out_scale);
   p.pre = static_cast<__nv_bfloat16*>(pre);
@@ -961,8 +975,10 @@ extern "C" int moe_grouped_gemm_fp8(const void* x, const void* x_scale, const vo
   p.most = 0x7fffffff;
   p.b_mn = w_kn ? 1 : 0;
   p.epilogue = epilogue;
-  p.x_words = p.num_kb % 4 == 0 && (reinterpret_cast<uintptr_t>(x_scale) & 3) == 0;
-  p.w_words = !w_kn && p.num_kb % 4 == 0 && (reinterpret_cast<uintptr_t>(w_scale) & 3) == 0;
+  p.xs = {static_cast<const uint8_t*>(x_scale), x_rows * p.num_kb, p.num_kb,
+          (reinterpret_cast<uintptr_t>(x_scale) & 3) == 0};
+  p.ws = {static_cast<const uint8_t*>(w_scale), num_w * p.n_blocks * p.num_kb, p.num_kb,
+          (reinterpret_cast<uintptr_t>(w_scale) & 3) == 0};
   CUtensorMap to, tp;
   st = g8::make_store_tmap(&to, out, static_cast<uint64_t>(epilogue == 1 ? p.f_half : p.n),
                            static_cast<uint64_t>(x_rows), epilogue == 0);
