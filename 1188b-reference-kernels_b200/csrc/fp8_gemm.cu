@@ -32,9 +32,9 @@
 // on a barrier of their own (`shared`), which the next tile's MMAs wait for;
 // the rest of a tile's epilogue overlaps the next tile's mainloop.
 // Measured (one B200 at its 1000 W, 1.2 to 1.5 GHz): 32 groups of 1024 rows,
-// K 7168, N 4096 with SwiGLU 0.89-0.93 ms, K 2048, N 7168 0.50-0.52 ms (2070
-// and 1860 TFLOP/s; power bounds both); 20 groups of one or two rows 119 us,
-// 4.9 TB/s of weights.
+// K 7168, N 4096 with SwiGLU 0.89-0.92 ms, K 2048, N 7168 0.49-0.52 ms (2100
+// and 1900 TFLOP/s; power bounds both); 20 groups of one or two rows 111-120 us,
+// 4.9-5.3 TB/s of weights.
 // Rows are described by the group table of moe_grouped_gemm_plan_*. Every
 // wait is bounded (2 s): on timeout the kernel records an error word, drains
 // its copies and MMAs, frees TMEM and returns.

@@ -19,7 +19,7 @@
 // Bound by instruction issue, about a thousand a token, and at the end by the
 // latency of a row that needs 64 bits (selected by a copy of c in shared
 // memory that took 10 us of 34): 16384 x 256, 8 groups of which 4 stay, top-8:
-// 29 us on the device against 6.0 us of bytes; 4 tokens: 4.8 us.
+// 28 us on the device against 6.0 us of bytes; 4 tokens: 4.8 us.
 // The gradient reads what a row needs and writes it once: 16384 x 256 from a
 // sigmoid 10 us (2.9 us of bytes).
 #include <math.h>
