@@ -220,7 +220,7 @@ MOE_DEVICE void load_scale_cells(const Params& p, int64_t row0, int64_t wi, int 
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     const int64_t r = row0 + c * 32 + lane;
-    a[c] = r < p.x_rows ? scale_cell(p.xs, r, kg) : 0x7F7F7F7Fu;
+    a[c] = static_cast<uint64_t>(r) < static_cast<uint64_t>(p.x_rows) ? scale_cell(p.xs, r, kg) : 0x7F7F7F7Fu;
   }
   if (p.b_mn) {  // bytes of one block lie a row of blocks apart: a lane loads each
     const int nb = lane & 4 ? nb1 : nb0;
@@ -419,7 +419,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int left = rows - tile.m_idx * kTileM;
         const int mine = left - static_cast<int>(rank) * 128;
         const CUtensorMap* map_a = kFew || mine <= kFewRows ? &tmap_a_few : &tmap_a;
-        const uint32_t bytes = a_bytes(left) + (kPair ? a_bytes(left - 128) + 2 * kTileBytes : 2 * kTileBytes);
+        // (the few form has room for the small box alone, whatever the table names)
+        const uint32_t bytes = a_bytes(kFew ? min(left, kFewRows) : left) + (kPair ? a_bytes(left - 128) + 2 * kTileBytes : 2 * kTileBytes);
         // A weight that one M-tile reads is not read again: it leaves L2
         // first (32 groups of 100 rows, K 2048: 122 -> 114 us).
         const uint64_t policy = rows <= kTileM ? l2_policy_evict_first() : l2_policy_evict_normal();
@@ -644,7 +645,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       const int m_local = tile.m_idx * kTileM + static_cast<int>(rank) * 128 + quad * 32 + lane;
       const int64_t row = static_cast<int64_t>(p.row_start[tile.g]) + m_local;
-      const bool rvalid = m_local < p.rows[tile.g] && row < p.x_rows;
+      const bool rvalid =
+          m_local < p.rows[tile.g] && static_cast<uint64_t>(row) < static_cast<uint64_t>(p.x_rows);
       // a warp whose 32 rows all belong to the group stores them with TMA
       const bool tma = !kFew && __all_sync(0xffffffffu, rvalid);
       const int warp_row0 = static_cast<int>(row) - lane;
@@ -910,7 +912,7 @@ extern "C" int moe_grouped_gemm_fp8(const void* x, const void* x_scale, const vo
   MOE_REQUIRE(epilogue == 0 || epilogue == 1, "grouped_gemm_fp8: epilogue must be 0 or 1");
   MOE_REQUIRE(G >= 1 && num_w >= 1, "grouped_gemm_fp8: G=%lld num_w=%lld", (long long)G,
               (long long)num_w);
-  MOE_REQUIRE(x_rows >= 0 && x_rows < (1ll << 31), "grouped_gemm_fp8: x_rows=%lld out of range",
+  MOE_REQUIRE(x_rows >= 0 && x_rows < (1ll << 31) - 256, "grouped_gemm_fp8: x_rows=%lld out of range",
               (long long)x_rows);
   MOE_REQUIRE(K >= 16 && K % 16 == 0 && K < (1ll << 31),
               "grouped_gemm_fp8: K=%lld must be a positive multiple of 16", (long long)K);
@@ -989,30 +991,30 @@ extern "C" int moe_grouped_gemm_fp8(const void* x, const void* x_scale, const vo
     if (st) return st;
   }
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (clusters > 0) {
+  // Calls of few rows stay with the one launch, which then takes every group (a
+  // table may name more rows than there are: those that are there count).
+  if (clusters > 0 && x_rows > g8::kSingleRows) {
     p.most = g8::kSingleRows;
-    if (x_rows > g8::kSingleRows) {
-      g8::Params pb = p;
-      pb.above = g8::kSingleRows;
-      pb.most = 0x7fffffff;
-      pb.n_chunk = static_cast<int>(
-          std::min<int64_t>(p.n_tiles, std::max<int64_t>(1, g8::kSlabBytes / (g8::BN * K))));
-      cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = dim3(2 * clusters);
-      cfg.blockDim = dim3(g8::kThreads);
-      cfg.dynamicSmemBytes = g8::Shape<g8::kPairForm>::kSmemBytes;
-      cfg.stream = s;
-      cudaLaunchAttribute attr[1];
-      attr[0].id = cudaLaunchAttributeClusterDimension;
-      attr[0].val.clusterDim.x = 2;
-      attr[0].val.clusterDim.y = 1;
-      attr[0].val.clusterDim.z = 1;
-      cfg.attrs = attr;
-      cfg.numAttrs = 1;
-      MOE_CUDA_CALL(
-          cudaLaunchKernelEx(&cfg, g8::grouped_gemm_fp8_kernel<g8::kPairForm>, ta, taf, tb, to, tp, pb),
-          "grouped_gemm_fp8 pair launch");
-    }
+    g8::Params pb = p;
+    pb.above = g8::kSingleRows;
+    pb.most = 0x7fffffff;
+    pb.n_chunk = static_cast<int>(
+        std::min<int64_t>(p.n_tiles, std::max<int64_t>(1, g8::kSlabBytes / (g8::BN * K))));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * clusters);
+    cfg.blockDim = dim3(g8::kThreads);
+    cfg.dynamicSmemBytes = g8::Shape<g8::kPairForm>::kSmemBytes;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    MOE_CUDA_CALL(
+        cudaLaunchKernelEx(&cfg, g8::grouped_gemm_fp8_kernel<g8::kPairForm>, ta, taf, tb, to, tp, pb),
+        "grouped_gemm_fp8 pair launch");
   }
   if (x_rows <= g8::kFewRows) {
     g8::grouped_gemm_fp8_kernel<g8::kFewForm>

@@ -234,7 +234,6 @@ def test_gemm_swiglu(cuda_dev, rows, g, n, k, with_pre):
 
 def test_gemm_rows_of_no_group_stay(cuda_dev):
     """Rows behind the last group, also inside its last tile, are not written."""
-    import ctypes  # noqa: F401
     import moe_b200
     from moe_b200 import _lib
     x, w = _operands(cuda_dev, 700, 2, 256, 256, "NK", 3)
@@ -333,6 +332,20 @@ def test_gemm_groups_that_share_weights(cuda_dev):
         d = (got[at:at + sum(counts[s])] - y).abs()
         assert bool((d <= 2.0 ** -8 * y.abs() + 1.01 * 384 * 2.0 ** -24 * m).all())
         at += sum(counts[s])
+
+
+@pytest.mark.parametrize("rows,splits", [(20, [40, 200]), (20, [5, 200]), (100, [40, 300]), (100, [300, 40]),
+                                         (140, [130, 900]), (300, [10, 5000])])
+def test_gemm_table_names_more_rows_than_there_are(cuda_dev, rows, splits):
+    """Splits on the device are not read on the host: the rows that exist get their group's product."""
+    import moe_b200
+    x, w = _operands(cuda_dev, rows, 2, 512, 384, "NK", 17)
+    plan = moe_b200.GroupedGemmPlan(2, cuda_dev).from_splits(torch.tensor(splits, device=cuda_dev))
+    y = moe_b200.grouped_gemm_fp8(x, w, plan=plan).double()
+    assert plan.device_error() == 0
+    first = min(splits[0], rows)
+    want, s = _product64(x, w, [first, rows - first], "NK")
+    assert bool(((y - want).abs() <= 2.0 ** -8 * want.abs() + 1.01 * 384 * 2.0 ** -24 * s).all())
 
 
 def test_offsets_past_32_bits(cuda_dev):
