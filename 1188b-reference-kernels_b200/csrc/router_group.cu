@@ -485,10 +485,12 @@ __global__ void __launch_bounds__(32 * kWarps) router_backward_kernel(
   float s = 0.f, g = 0.f;
   if (lane < k) {
     const int64_t slot = __ldg(idx + t * k + lane);
-    if (slot >= 0 && slot < E) {
-      col = perm ? __ldg(perm + slot) : static_cast<int>(slot);
+    if (slot >= 0 && slot < E) col = perm ? __ldg(perm + slot) : static_cast<int>(slot);
+    if (col >= 0 && col < E) {
       g = scale * (grad_vals ? __ldg(grad_vals + t * k + lane) : __ldg(grad_probs + t * E + slot));
       s = score(col);
+    } else {
+      col = -1;  // named by neither the list nor the placement: no gradient
     }
   }
   if (list_softmax) {

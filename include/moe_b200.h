@@ -127,9 +127,9 @@ int moe_router_group_topk(const float* logits, const float* bias, int64_t T, int
 /* s_e (ds_e - sum_j ds_j s_j). Exactly one of grad_vals [T,k] and grad_probs */
 /* [T,E] (read at the selected entries alone) is given. placement: as in      */
 /* moe_router_topk_placed (topk_idx and grad_probs count slots; bias and      */
-/* grad_logits model experts). An index outside [0,E) is skipped; an expert   */
-/* named twice gets the sum of its gradients. grad_logits [T,E] fp32 is       */
-/* written whole. k <= 32.                                                    */
+/* grad_logits model experts). An index or a placement outside [0,E) is       */
+/* skipped; an expert named twice gets the sum of its gradients. grad_logits  */
+/* [T,E] fp32 is written whole. k <= 32.                                      */
 int moe_router_topk_backward(const float* logits, const float* bias, const int32_t* placement,
                              const int64_t* topk_idx, const float* grad_vals,
                              const float* grad_probs, int64_t T, int64_t E, int32_t k,

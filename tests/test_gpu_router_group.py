@@ -254,6 +254,22 @@ def test_backward_placement(cuda_dev):
     assert torch.equal(got[:, perm], want)
 
 
+@pytest.mark.parametrize("score,renorm", [("sigmoid", True), ("softmax", False), ("softmax", True)])
+def test_backward_placement_out_of_range(cuda_dev, score, renorm):
+    """A slot whose placement names no expert is one that the list does not name."""
+    import moe_b200
+    t, e, k = 5, 8, 3
+    x, idx, gv = (v.to(cuda_dev) for v in _bwd_case(t, e, k, 9, False))
+    pl = torch.arange(e, dtype=torch.int32, device=cuda_dev)
+    pl[2], pl[5] = -1, e + 100
+    kw = dict(grad_vals=gv, score=score, renorm=renorm)
+    got = moe_b200.router_topk_backward(x, idx, placement=pl, **kw)
+    gone = (idx == 2) | (idx == 5)
+    assert bool(gone.any())
+    want = moe_b200.router_topk_backward(x, torch.where(gone, torch.full_like(idx, -1), idx), **kw)
+    assert torch.equal(got, want)
+
+
 def test_router_in_a_graph(cuda_dev):
     import moe_b200
     x = torch.randn(100, 64, device=cuda_dev)
