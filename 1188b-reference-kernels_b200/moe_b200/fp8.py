@@ -177,6 +177,8 @@ def grouped_gemm_fp8(x: Fp8Tensor, w: Fp8Tensor,
     rows, k = x.data.shape
     g, d1, d2 = w.data.shape
     n = d1 if w_layout == "NK" else d2
+    if g < 1:
+        raise ValueError("w holds no weight matrix")
     _need_k("x.data", k)
     _need_fp8("x", x, (rows, _blocks(k)))
     _need_fp8("w", w, (g, _blocks(d1), _blocks(d2)))
@@ -193,9 +195,12 @@ def grouped_gemm_fp8(x: Fp8Tensor, w: Fp8Tensor,
         if not isinstance(m_splits, torch.Tensor):
             if len(m_splits) != g:
                 raise ValueError(f"m_splits has {len(m_splits)} entries for {g} groups")
-            if sum(int(v) for v in m_splits) > rows:
+            m_splits = [int(v) for v in m_splits]
+            if min(m_splits) < 0:
+                raise ValueError(f"m_splits must not be negative, got {min(m_splits)}")
+            if sum(m_splits) > rows:
                 raise ValueError("sum(m_splits) exceeds x rows")
-            m_splits = torch.tensor([int(v) for v in m_splits], dtype=torch.int32)
+            m_splits = torch.tensor(m_splits, dtype=torch.int32)
         with _on(dev):
             plan = GroupedGemmPlan(g, dev).from_splits(m_splits)
     if plan.num_w != g or plan.workspace.device != dev:

@@ -140,6 +140,8 @@ def test_ops_refuse_bad_shapes(cuda_dev):
            lambda: moe_b200.grouped_gemm_fp8(q, w, return_pre=True),
            lambda: moe_b200.grouped_gemm_fp8(q, w, w_layout="KN"),
            lambda: moe_b200.grouped_gemm_fp8(q, moe_b200.Fp8Tensor(w.data, w.scale[:, :0])),
+           lambda: moe_b200.grouped_gemm_fp8(q, w, [-1, 5]),
+           lambda: moe_b200.grouped_gemm_fp8(q, moe_b200.Fp8Tensor(w.data[:0], w.scale[:0])),
            lambda: moe_b200.grouped_gemm_fp8(q, w, epilogue="fp32")]
     for i, call in enumerate(bad):
         with pytest.raises(ValueError):
