@@ -16,10 +16,12 @@
 // One warp per token: a row is a kilobyte, its group maxima and its selection
 // are exchanges between lanes, and nothing has to leave the warp. A lane
 // holds consecutive columns of one group, so that a group is a few lanes.
-// Bound by instruction issue, about a thousand a token, and at the end by the
-// latency of a row that needs 64 bits (selected by a copy of c in shared
-// memory that took 10 us of 34): 16384 x 256, 8 groups of which 4 stay, top-8:
-// 28 us on the device against 6.0 us of bytes; 4 tokens: 4.8 us.
+// Bound by instruction issue, and at the end by the latency of a row that
+// needs 64 bits (without them 3 us less; selected by a copy of c in shared
+// memory they took 10 us of 34): 16384 x 256, 8 groups of which 4 stay, top-8:
+// 24.5 us on the device against 6.0 us of bytes (28.5 with __expf and
+// __fdividef, which cover subnormal numbers, and with checks of every column);
+// 8192 x 1024, one group: 48 us; 4 tokens: 4.8 us.
 // The gradient reads what a row needs and writes it once: 16384 x 256 from a
 // sigmoid 10 us (2.9 us of bytes).
 #include <math.h>
@@ -146,13 +148,30 @@ MOE_DEVICE int select64(const Scores64& sc, double* c, int E, int k, int groups,
   return mine;
 }
 
-// Order-preserving bits of a float that is no NaN (-0 equal to +0); never 0.
+// Order-preserving bits of a float that is neither NaN nor -0; never 0.
 MOE_DEVICE uint32_t order_key32(float v) {
-  const uint32_t u = __float_as_uint(v + 0.0f);
-  return (u >> 31) ? ~u : (u | 0x80000000u);
+  const uint32_t u = __float_as_uint(v);
+  return u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
 }
 MOE_DEVICE float key32_value(uint32_t key) {
   return __uint_as_float((key >> 31) ? (key & 0x7fffffffu) : ~key);
+}
+
+// One instruction each; subnormal results are 0.
+MOE_DEVICE float fast_exp(float t) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t * 1.4426950408889634f));
+  return r;
+}
+MOE_DEVICE float fast_rcp(float y) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(y));
+  return r;
+}
+MOE_DEVICE float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 
 struct RouteArgs {
@@ -174,20 +193,36 @@ struct RouteArgs {
 // `err` (below), so an order of fp32 values is the true one where neighbours
 // differ by more than 2 err. Returns false, in every lane, where a decision
 // hangs on less than that (0.5 % of the rows of normal logits), or at a NaN;
-// the caller then selects in 64 bits.
-template <int VPL>
+// the caller then selects in 64 bits. kFull: every lane holds VPL columns, a
+// multiple of 4, and the rows are 16-byte aligned.
+template <int VPL, bool kFull>
 MOE_DEVICE bool select32(const RouteArgs& a, const float* x, int* s_mine, int& mine) {
   const int lane = lane_id();
   const int size = a.E / a.groups;
   const int g = lane / a.lanes;
   const int first = (lane & (a.lanes - 1)) * a.vpl;  // inside the group
-  const int n = g < a.groups ? max(0, min(a.vpl, size - first)) : 0;
+  const int n = kFull ? VPL : g < a.groups ? max(0, min(a.vpl, size - first)) : 0;
   const int col0 = g * size + first;
-  float v[VPL], c[VPL];
+  float v[VPL], c[VPL], add[VPL];
+  auto load = [&](const float* p, float none, float (&r)[VPL]) {
+    if constexpr (kFull) {
 #pragma unroll
-  for (int j = 0; j < VPL; ++j) v[j] = j < n ? __ldg(x + col0 + j) : -INFINITY;
+      for (int j = 0; j < VPL; j += 4) {
+        const float4 q = __ldg(reinterpret_cast<const float4*>(p + col0 + j));
+        r[j] = q.x;
+        r[j + 1] = q.y;
+        r[j + 2] = q.z;
+        r[j + 3] = q.w;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) r[j] = j < n ? __ldg(p + col0 + j) : none;
+    }
+  };
+  load(x, -INFINITY, v);
+  if (a.bias != nullptr) load(a.bias, 0.f, add);
   // fp32 scores and what they may be off by, in units of 2^-23.
-  // __expf(t) is off by 2 + 1.18 |t| of itself, __fdividef by 2.
+  // fast_exp(t) is off by 2 + 1.18 |t| of itself, fast_rcp by 1, its use by 1.
   // sigmoid: of exp's error s (1 - s) arrives, at most 1/4 * 2 + 1.18 * 0.23;
   //   the sum 1 + e adds 1/2, the quotient 2: together below 4.
   // softmax: t = x - m adds |t| / 2 to exp's; s |t| <= 1/e (z >= 1), so
@@ -203,8 +238,8 @@ MOE_DEVICE bool select32(const RouteArgs& a, const float* x, int* s_mine, int& m
     m = warp_maxf(m);
     float z = 0.f;
 #pragma unroll
-    for (int j = 0; j < VPL; ++j) z += j < n ? __expf(v[j] - m) : 0.f;
-    rz = __fdividef(1.0f, warp_sumf(z));
+    for (int j = 0; j < VPL; ++j) z += kFull || j < n ? fast_exp(v[j] - m) : 0.f;
+    rz = fast_rcp(warp_sumf(z));
     err = (1.f + 30.f * rz) * 1.1920929e-7f;
   } else {
     err = 4.f * 1.1920929e-7f;
@@ -213,16 +248,21 @@ MOE_DEVICE bool select32(const RouteArgs& a, const float* x, int* s_mine, int& m
   float big = 0.f;
 #pragma unroll
   for (int j = 0; j < VPL; ++j) {
-    c[j] = a.softmax ? __expf(v[j] - m) * rz : __fdividef(1.0f, 1.0f + __expf(-v[j]));
-    if (a.bias != nullptr && j < n) c[j] += __ldg(a.bias + col0 + j);
-    if (j < n) {
-      odd |= isnan(c[j]);
-      if (c[j] > -INFINITY) big = fmaxf(big, fabsf(c[j]));  // a bias of -inf is exact
-    }
+    c[j] = a.softmax ? fast_exp(v[j] - m) * rz : fast_rcp(1.0f + fast_exp(-v[j]));
+    if (a.bias != nullptr) c[j] += add[j];
+    big = max_nan(big, fabsf(c[j]));
   }
-  // __fdividef(1, y) is 0 for y in (2^126, inf), as sigmoid of such x is to
-  // within 2^-126
+  // (columns that are not there have c = 0). Of a y above 2^126 the reciprocal
+  // is 0, as sigmoid of such x is to within 2^-126.
   big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big)));
+  if (!(big < INFINITY)) {
+    odd |= isnan(big);
+    big = 0.f;  // a bias of -inf is exact
+#pragma unroll
+    for (int j = 0; j < VPL; ++j)
+      if (c[j] > -INFINITY) big = fmaxf(big, fabsf(c[j]));
+    big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big)));
+  }
   err += 5.9604645e-8f * big;
   const float gap = 2.f * err;
 
@@ -231,7 +271,7 @@ MOE_DEVICE bool select32(const RouteArgs& a, const float* x, int* s_mine, int& m
     float hi = -INFINITY, lo = -INFINITY;
 #pragma unroll
     for (int j = 0; j < VPL; ++j)
-      if (j < n) {
+      if (kFull || j < n) {
         lo = fmaxf(lo, fminf(hi, c[j]));
         hi = fmaxf(hi, c[j]);
       }
@@ -257,7 +297,7 @@ MOE_DEVICE bool select32(const RouteArgs& a, const float* x, int* s_mine, int& m
   }
   uint32_t key[VPL];
 #pragma unroll
-  for (int j = 0; j < VPL; ++j) key[j] = in && j < n && !odd ? order_key32(c[j]) : 0u;
+  for (int j = 0; j < VPL; ++j) key[j] = in && (kFull || j < n) && !odd ? order_key32(c[j]) : 0u;
   // A lane offers its best column; its second best stands ready, and only a
   // lane that wins a third time looks through its columns again.
   uint32_t b1 = 0, b2 = 0;
@@ -271,13 +311,14 @@ MOE_DEVICE bool select32(const RouteArgs& a, const float* x, int* s_mine, int& m
     c1 = first ? j : c1;
   }
   bool spare = true;
+  uint32_t wins = 0;
   uint32_t won = 0;                 // lane r: the key of round r
   for (int r = 0; r <= a.k; ++r) {  // one more than is taken: the border below
     const uint32_t w = __reduce_max_sync(0xffffffffu, b1);
     if (lane == r) won = w;
     if (w == 0u || r == a.k) break;  // nothing left (all taken, or a NaN: odd)
-    const int owner = __ffs(__ballot_sync(0xffffffffu, b1 == w)) - 1;
-    if (lane == owner) {
+    if (b1 == w) {  // one lane, or several of equal keys: the wins then add up to more than k
+      ++wins;
       s_mine[r] = col0 + c1;
       if (spare) {
         b1 = b2;
@@ -296,8 +337,9 @@ MOE_DEVICE bool select32(const RouteArgs& a, const float* x, int* s_mine, int& m
   }
   __syncwarp();
   mine = lane < a.k ? s_mine[lane] : 0;
-  // Rounds whose keys lie too close (equal ones, of two lanes or of one, come
-  // up in consecutive rounds) leave their order open; so does an empty round.
+  odd |= __reduce_add_sync(0xffffffffu, wins) != static_cast<uint32_t>(a.k);
+  // Rounds whose keys lie too close (equal ones of one lane come up in
+  // consecutive rounds) leave their order open; so does an empty round.
   const uint32_t before = __shfl_up_sync(0xffffffffu, won, 1);
   if (lane < a.k) odd |= won == 0u;
   if (lane >= 1 && lane <= a.k && won != 0u) odd |= !(key32_value(before) - key32_value(won) > gap);
@@ -381,8 +423,9 @@ MOE_DEVICE int select64_lanes(const RouteArgs& a, const Scores64& sc, int* s_min
 }
 
 // One warp per token. VPL 0: 64 bits throughout, the scores in shared memory
-// (shapes whose lanes would hold more than 16 columns).
-template <int VPL>
+// (shapes whose lanes would hold more than 32 columns: 17 to 31 groups that
+// leave lanes without any).
+template <int VPL, bool kFull>
 __global__ void __launch_bounds__(32 * kWarps) router_group_kernel(const RouteArgs a) {
   extern __shared__ double s_c[];
   const int lane = lane_id();
@@ -407,7 +450,7 @@ __global__ void __launch_bounds__(32 * kWarps) router_group_kernel(const RouteAr
   int mine = 0;
   bool done = false;
   __shared__ int s_mine[kWarps][kMaxK];
-  if constexpr (VPL > 0) done = select32<VPL>(a, x, s_mine[warp_id()], mine);
+  if constexpr (VPL > 0) done = select32<VPL, kFull>(a, x, s_mine[warp_id()], mine);
   Scores64 sc{x, a.bias, 0.0, 1.0, a.softmax != 0, false};
   // The softmax's normaliser cancels in renormalised weights, so that only
   // the 64-bit selection and plain softmax weights need it.
@@ -441,8 +484,18 @@ __global__ void __launch_bounds__(32 * kWarps) router_group_kernel(const RouteAr
 
 template <int VPL>
 void launch_route(const RouteArgs& a, cudaStream_t s) {
-  router_group_kernel<VPL><<<static_cast<unsigned>((a.T + kWarps - 1) / kWarps), 32 * kWarps,
-                             VPL > 0 ? 0 : kWarps * a.E * sizeof(double), s>>>(a);
+  const unsigned grid = static_cast<unsigned>((a.T + kWarps - 1) / kWarps);
+  if constexpr (VPL >= 4 && VPL % 4 == 0) {
+    // every lane full: no column is asked whether it is there, and loads are of 16 bytes (8 groups of 32:
+    // 24.8 against 27.2 us, 16 of 32: 36 against 51)
+    if (a.E == 32 * VPL && 32 / a.lanes == a.groups && a.vpl == VPL &&
+        ((reinterpret_cast<uintptr_t>(a.logits) | reinterpret_cast<uintptr_t>(a.bias)) & 15) == 0) {
+      router_group_kernel<VPL, true><<<grid, 32 * kWarps, 0, s>>>(a);
+      return;
+    }
+  }
+  router_group_kernel<VPL, false>
+      <<<grid, 32 * kWarps, VPL > 0 ? 0 : kWarps * a.E * sizeof(double), s>>>(a);
 }
 
 // One warp per token; lane j < k holds the j-th selected expert.
@@ -596,6 +649,8 @@ extern "C" int moe_router_group_topk(const float* logits, const float* bias, int
     launch_route<12>(a, s);
   else if (a.vpl <= 16)
     launch_route<16>(a, s);
+  else if (a.vpl <= 32)
+    launch_route<32>(a, s);
   else
     launch_route<0>(a, s);
   MOE_CUDA_CHECK_LAUNCH("router_group_topk launch");

@@ -232,6 +232,24 @@ def test_gemm_swiglu(cuda_dev, rows, g, n, k, with_pre):
     _check_swiglu(q, pre, *_product64(x, w, splits, "NK"), k)
 
 
+@pytest.mark.parametrize("splits", [[1], [4], [5], [32], [0, 31, 1], [12, 0, 11, 3], [1] * 9 + [0] * 20])
+@pytest.mark.parametrize("n,k,layout", [(256, 4112, "NK"), (264, 2048, "NK"), (2560, 1040, "NK"), (528, 4608, "KN")])
+def test_gemm_few_rows(cuda_dev, splits, n, k, layout):
+    """Calls of at most 32 rows share the K range of a tile between CTAs (K of 3 to 9 groups of 512)."""
+    import moe_b200
+    rows, g = sum(splits), len(splits)
+    x, w = _operands(cuda_dev, rows, g, n, k, layout, rows + k)
+    plan = moe_b200.GroupedGemmPlan(g, cuda_dev).from_splits(torch.tensor(splits))
+    got = [moe_b200.grouped_gemm_fp8(x, w, plan=plan, w_layout=layout) for _ in range(3)]
+    y, s = _product64(x, w, splits, layout)
+    assert plan.device_error() == 0
+    assert bool(((got[0].double() - y).abs() <= 2.0 ** -8 * y.abs() + 1.01 * k * 2.0 ** -24 * s).all())
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+    if layout == "NK" and n % 256 == 0:
+        q, pre = moe_b200.grouped_gemm_fp8(x, w, plan=plan, epilogue="swiglu_fp8", return_pre=True)
+        _check_swiglu(q, pre, y, s, k)
+
+
 def test_gemm_rows_of_no_group_stay(cuda_dev):
     """Rows behind the last group, also inside its last tile, are not written."""
     import moe_b200

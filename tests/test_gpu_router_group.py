@@ -112,6 +112,32 @@ def test_route_masked_logits(cuda_dev, score, renorm):
         assert bool(torch.isfinite(r.probs).all())
 
 
+@pytest.mark.parametrize("e,groups,keep,k", [(128, 1, 1, 4), (128, 16, 5, 8), (256, 8, 4, 8), (384, 1, 1, 8),
+                                             (384, 32, 7, 6), (512, 16, 4, 8), (1024, 1, 1, 16), (1024, 32, 3, 9),
+                                             (1020, 17, 5, 6)])
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+def test_route_wide_rows(cuda_dev, e, groups, keep, k, score):
+    """Every layout of a row over the lanes: ties, near ties, masked logits, a bias that bars experts,
+    unaligned rows."""
+    import moe_b200
+    t = 48
+    g = torch.Generator().manual_seed(e + groups)
+    x = torch.randn(t, e, generator=g) * 3
+    ties = torch.randint(0, 40, (t, e), generator=g).float() / 8
+    near = 1.0 + torch.randint(0, 64, (t, e), generator=g) * 2.0 ** -23
+    masked = torch.where(torch.rand(t, e, generator=g) < 0.97, torch.full((t, e), -float("inf")), x)
+    far = x * 40  # saturated and vanishing scores
+    bar = torch.where(torch.rand(e, generator=g) < 0.3, torch.full((e,), -float("inf")), torch.zeros(e))
+    small = torch.randint(-2, 3, (e,), generator=g).float() * 2.0 ** -6
+    store = torch.empty(t * e + 1, device=cuda_dev)
+    for logits in (x, ties, near, masked, far):
+        for bias in (None, bar, small):
+            for view in (logits.to(cuda_dev), store[1:].view(t, e).copy_(logits)):
+                r = moe_b200.router_group_topk(view, k, score=score, num_groups=groups, topk_groups=keep,
+                                               bias=None if bias is None else bias.to(cuda_dev), scale=0.5)
+                _check(r, *route64(logits, k, score, groups, keep, "top2", bias, True, 0.5), e)
+
+
 def test_route_nan_row_stays_in_its_row(cuda_dev):
     import moe_b200
     x = torch.randn(6, 32, generator=torch.Generator().manual_seed(1))
