@@ -23,8 +23,10 @@
 // __fdividef, which cover subnormal numbers, and with checks of every column);
 // 8192 x 1024, one group: 48 us; 4 tokens: 4.8 us.
 // The gradient reads what a row needs and writes it once: 16384 x 256 from a
-// sigmoid 10 us (2.9 us of bytes).
+// sigmoid 7.7 us (2.9 us of bytes; 9.8 with a warp a token).
 #include <math.h>
+
+#include <type_traits>
 
 #include "moe_common.cuh"
 
@@ -498,25 +500,44 @@ void launch_route(const RouteArgs& a, cudaStream_t s) {
       <<<grid, 32 * kWarps, VPL > 0 ? 0 : kWarps * a.E * sizeof(double), s>>>(a);
 }
 
-// One warp per token; lane j < k holds the j-th selected expert.
+// kLanes lanes per token, of which lane j < k holds the j-th selected expert.
 //   renorm: ds_j = scale * (g_j / S - (sum_i g_i s_i) / S^2), S = sum_i s_i;  else ds_j = scale * g_j
 //   sigmoid: dx_j = ds_j s_j (1 - s_j), 0 elsewhere; logits: dx_j = ds_j
 //   softmax: dx_e = s_e (ds_e - sum_j ds_j s_j), ds 0 outside the selection
 // With renorm the softmax's normaliser cancels: the weights are a softmax w of
 // the selected logits alone, dx_j = w_j (g_j - sum_i g_i w_i), exactly 0
 // elsewhere, and the rest of the row is not read.
+// What a token waits for is its list, then the gathers; with as few lanes a
+// token as its list needs, a warp has those of several under way.
+template <int kLanes>
+MOE_DEVICE float group_sum(float v) {
+#pragma unroll
+  for (int off = kLanes / 2; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  return v;
+}
+template <int kLanes>
+MOE_DEVICE float group_max(float v) {
+#pragma unroll
+  for (int off = kLanes / 2; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
+  return v;
+}
+
+template <int kLanes>
 __global__ void __launch_bounds__(32 * kWarps) router_backward_kernel(
     const float* __restrict__ logits, const float* __restrict__ bias,
     const int32_t* __restrict__ perm, const int64_t* __restrict__ idx,
     const float* __restrict__ grad_vals, const float* __restrict__ grad_probs, int64_t T, int E,
     int k, int mode, int renorm, float scale, float* __restrict__ out) {
+  constexpr int kTokens = 32 / kLanes;  // of a warp
   const int lane = lane_id();
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * kWarps + warp_id();
-  if (t >= T) return;
+  const int l = lane % kLanes;
+  const int64_t t0 = (static_cast<int64_t>(blockIdx.x) * kWarps + warp_id()) * kTokens;
+  if (t0 >= T) return;
+  const int64_t t = t0 + lane / kLanes;
   const float* x = logits + t * E;
   float* o = out + t * E;
   const bool list_softmax = mode == 1 && renorm;
-  const bool row_softmax = mode == 1 && !renorm;
+  const bool row_softmax = kLanes == 32 && mode == 1 && !renorm;
   float m = 0.f, z = 1.f;
   if (row_softmax) {
     m = -INFINITY;
@@ -536,44 +557,49 @@ __global__ void __launch_bounds__(32 * kWarps) router_backward_kernel(
   };
   int col = -1;  // this lane's expert, as a column of the logits
   float s = 0.f, g = 0.f;
-  if (lane < k) {
-    const int64_t slot = __ldg(idx + t * k + lane);
+  if (l < k && t < T) {
+    const int64_t slot = __ldg(idx + t * k + l);
     if (slot >= 0 && slot < E) col = perm ? __ldg(perm + slot) : static_cast<int>(slot);
     if (col >= 0 && col < E) {
-      g = scale * (grad_vals ? __ldg(grad_vals + t * k + lane) : __ldg(grad_probs + t * E + slot));
+      g = scale * (grad_vals ? __ldg(grad_vals + t * k + l) : __ldg(grad_probs + t * E + slot));
       s = score(col);
     } else {
       col = -1;  // named by neither the list nor the placement: no gradient
     }
   }
   if (list_softmax) {
-    m = warp_maxf(col >= 0 ? s : -INFINITY);
+    m = group_max<kLanes>(col >= 0 ? s : -INFINITY);
     s = col >= 0 && m > -INFINITY ? expf(s - m) : 0.f;
-    const float S = warp_sumf(s);
+    const float S = group_sum<kLanes>(s);
     s = S == 0.f ? 0.f : s / S;
   }
   float ds = g;
   if (list_softmax) {
-    ds = g - warp_sumf(g * s);
+    ds = g - group_sum<kLanes>(g * s);
   } else if (renorm) {
-    const float S = warp_sumf(s);
-    const float dot = warp_sumf(g * s);
+    const float S = group_sum<kLanes>(s);
+    const float dot = group_sum<kLanes>(g * s);
     ds = S == 0.f ? 0.f : g / S - dot / (S * S);
   }
   const float dot = row_softmax ? warp_sumf(ds * s) : 0.f;
   // an expert named twice gets the sum of its gradients
   float dsum = 0.f;
   for (int j = 0; j < k; ++j) {
-    const int cj = __shfl_sync(0xffffffffu, col, j);
-    const float dj = __shfl_sync(0xffffffffu, ds, j);
+    const int cj = __shfl_sync(0xffffffffu, col, j, kLanes);
+    const float dj = __shfl_sync(0xffffffffu, ds, j, kLanes);
     if (cj == col) dsum += dj;
   }
-  if (row_softmax)
+  if (row_softmax) {
     for (int e = lane; e < E; e += 32) o[e] = -score(e) * dot;
-  else if (E % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0)
-    for (int e = lane; e < E / 4; e += 32) reinterpret_cast<float4*>(o)[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-  else
-    for (int e = lane; e < E; e += 32) o[e] = 0.f;
+  } else {  // the warp's rows lie one behind the other
+    float* first = out + t0 * E;
+    const int64_t values = (T - t0 < kTokens ? T - t0 : kTokens) * E;
+    if (E % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0)
+      for (int64_t e = lane; e < values / 4; e += 32)
+        reinterpret_cast<float4*>(first)[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+    else
+      for (int64_t e = lane; e < values; e += 32) first[e] = 0.f;
+  }
   __syncwarp();
   if (col >= 0) {
     float d = dsum;
@@ -582,6 +608,13 @@ __global__ void __launch_bounds__(32 * kWarps) router_backward_kernel(
     if (list_softmax) d = s * dsum;
     o[col] = d;
   }
+}
+
+template <int kLanes, typename... Args>
+void launch_backward(int64_t T, cudaStream_t s, Args... args) {
+  const int64_t tokens = kWarps * (32 / kLanes);  // of a CTA
+  router_backward_kernel<kLanes>
+      <<<static_cast<unsigned>((T + tokens - 1) / tokens), 32 * kWarps, 0, s>>>(args...);
 }
 
 }  // namespace
@@ -672,10 +705,17 @@ extern "C" int moe_router_topk_backward(const float* logits, const float* bias,
   if (T == 0) return MOE_OK;
   MOE_REQUIRE(logits && topk_idx && grad_logits, "router_topk_backward: null pointer");
   MOE_REQUIRE(T <= (int64_t)0x7fffffff * kWarps, "router_topk_backward: T too large");
-  router_backward_kernel<<<static_cast<unsigned>((T + kWarps - 1) / kWarps), 32 * kWarps, 0,
-                           reinterpret_cast<cudaStream_t>(stream)>>>(
-      logits, bias, placement, topk_idx, grad_vals, grad_probs, T, static_cast<int>(E), k,
-      score_mode, renorm, scale, grad_logits);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  auto launch = [&](auto lanes) {
+    launch_backward<decltype(lanes)::value>(T, s, logits, bias, placement, topk_idx, grad_vals, grad_probs,
+                                            T, static_cast<int>(E), k, score_mode, renorm, scale, grad_logits);
+  };
+  if (k > 16 || (score_mode == 1 && !renorm))  // or the whole row is read
+    launch(std::integral_constant<int, 32>());
+  else if (k > 8)
+    launch(std::integral_constant<int, 16>());
+  else
+    launch(std::integral_constant<int, 8>());
   MOE_CUDA_CHECK_LAUNCH("router_topk_backward launch");
   return MOE_OK;
 }

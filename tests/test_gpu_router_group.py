@@ -179,7 +179,8 @@ def _bwd_case(t, e, k, seed, positive):
     return x, idx, torch.randn(t, k, generator=g)
 
 
-@pytest.mark.parametrize("t,e,k", [(1, 1, 1), (3, 8, 2), (65, 160, 6), (200, 256, 8), (7, 64, 32), (5, 1500, 3)])
+@pytest.mark.parametrize("t,e,k", [(1, 1, 1), (3, 8, 2), (65, 160, 6), (200, 256, 8), (7, 64, 32), (5, 1500, 3),
+                                   (37, 50, 12), (9, 20, 16)])
 @pytest.mark.parametrize("score", ["sigmoid", "softmax", "logits"])
 @pytest.mark.parametrize("renorm", [False, True])
 @pytest.mark.parametrize("dense", [False, True])
