@@ -32,8 +32,8 @@
 // on a barrier of their own (`shared`), which the next tile's MMAs wait for;
 // the rest of a tile's epilogue overlaps the next tile's mainloop.
 // Measured (one B200 at its 1000 W, 1.2 to 1.5 GHz): 32 groups of 1024 rows,
-// K 7168, N 4096 with SwiGLU 0.89-0.92 ms, K 2048, N 7168 0.49-0.52 ms (2100
-// and 1900 TFLOP/s; power bounds both); 20 groups of one or two rows 111-120 us,
+// K 7168, N 4096 with SwiGLU 0.88-0.92 ms, K 2048, N 7168 0.48-0.51 ms (2150
+// and 1950 TFLOP/s; power bounds both); 20 groups of one or two rows 111-120 us,
 // 4.9-5.3 TB/s of weights.
 // Rows are described by the group table of moe_grouped_gemm_plan_*. Every
 // wait is bounded (2 s): on timeout the kernel records an error word, drains
@@ -85,6 +85,11 @@ constexpr uint32_t kSfCol = 480;    // TMEM columns of the scales: 4 for A, 8 fo
 // 100 rows (K 7168, N 4096): 183 us single, 217 pair; 40 of 200 ([K,N], K 4096,
 // N 5120): 253 single, 229 pair.
 constexpr int kSingleRows = 128;
+// Calls of at least so many rows a group on average leave small groups to the
+// pairs as well, and make one launch (K 2048, N 7168: 32 groups of 1024 rows 430
+// -> 418 us, 16 of 100 and 924 in turn 157 -> 141, 30 of 4 rows beside 2 of 8132
+// 298 and 300; K 7168, N 4096: one of 1024 42 -> 39, 16 of 100 and 924 252 -> 255).
+constexpr int64_t kOneLaunchRows = 512;
 constexpr int64_t kSlabBytes = 32ll << 20;  // weight bytes walked per pass: they stay in L2 beside the rows
 
 constexpr int kErrProducer = 1;
@@ -393,6 +398,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   if constexpr (kPair) cluster_sync();  // barriers of both CTAs initialised before any remote use
   tc_fence_after();
   const uint32_t tmem = uniform(*tmem_slot);
+  // The single form's launch behind this one works on other groups: its CTAs
+  // start where this one's have left ([K,N], K 4096, N 5120, 40 groups of 20 to
+  // 380 rows: 291 -> 278 us).
+  if constexpr (kPair) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int groups4 = (p.num_kb + 3) / 4;
 
   gg::WalkerRT<kTileM> walker{p.rows, p.G, p.n_tiles, 1 << 20, p.n_chunk, p.above, p.most};
@@ -805,6 +814,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     else
       tmem_dealloc(tmem, kTmemCols);
   }
+  // What follows in the stream waits for this launch alone, so it ends after the pairs'.
+  if constexpr (!kPair) asm volatile("griddepcontrol.wait;" ::: "memory");
   // Neither SM is given to another kernel's CTA, which allocates TMEM, before
   // both have released the pair's.
   if constexpr (kPair) cluster_sync();
@@ -993,10 +1004,12 @@ extern "C" int moe_grouped_gemm_fp8(const void* x, const void* x_scale, const vo
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   // Calls of few rows stay with the one launch, which then takes every group (a
   // table may name more rows than there are: those that are there count).
-  if (clusters > 0 && x_rows > g8::kSingleRows) {
+  const bool pairs = clusters > 0 && x_rows > g8::kSingleRows;
+  const bool one_launch = pairs && x_rows >= g8::kOneLaunchRows * G;
+  if (pairs) {
     p.most = g8::kSingleRows;
     g8::Params pb = p;
-    pb.above = g8::kSingleRows;
+    pb.above = one_launch ? 0 : g8::kSingleRows;
     pb.most = 0x7fffffff;
     pb.n_chunk = static_cast<int>(
         std::min<int64_t>(p.n_tiles, std::max<int64_t>(1, g8::kSlabBytes / (g8::BN * K))));
@@ -1015,6 +1028,7 @@ extern "C" int moe_grouped_gemm_fp8(const void* x, const void* x_scale, const vo
     MOE_CUDA_CALL(
         cudaLaunchKernelEx(&cfg, g8::grouped_gemm_fp8_kernel<g8::kPairForm>, ta, taf, tb, to, tp, pb),
         "grouped_gemm_fp8 pair launch");
+    if (one_launch) return MOE_OK;
   }
   if (x_rows <= g8::kFewRows) {
     g8::grouped_gemm_fp8_kernel<g8::kFewForm>
@@ -1022,8 +1036,18 @@ extern "C" int moe_grouped_gemm_fp8(const void* x, const void* x_scale, const vo
     MOE_CUDA_CHECK_LAUNCH("grouped_gemm_fp8 few launch");
     return MOE_OK;
   }
-  g8::grouped_gemm_fp8_kernel<g8::kSingleForm>
-      <<<num_sms(dev), g8::kThreads, g8::Shape<g8::kSingleForm>::kSmemBytes, s>>>(ta, taf, tb, to, tp, p);
-  MOE_CUDA_CHECK_LAUNCH("grouped_gemm_fp8 launch");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(num_sms(dev));
+  cfg.blockDim = dim3(g8::kThreads);
+  cfg.dynamicSmemBytes = g8::Shape<g8::kSingleForm>::kSmemBytes;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pairs ? 1 : 0;  // a launch that follows another's kernel waits for its end
+  MOE_CUDA_CALL(
+      cudaLaunchKernelEx(&cfg, g8::grouped_gemm_fp8_kernel<g8::kSingleForm>, ta, taf, tb, to, tp, p),
+      "grouped_gemm_fp8 launch");
   return MOE_OK;
 }

@@ -129,7 +129,7 @@ EXPORTED = tuple(_SIGNATURES)
 # tiles, then the single-CTA kernel on the group remainders (one launch only
 # when CTA pairs are disabled with MOE_GEMM_PAIR=0 or MOE_GEMM_SPLIT=0). The
 # 8-bit one counts the launch that every call makes; calls of more than 128
-# rows make a second.
+# rows, but fewer than 512 a group, make a second.
 _LAUNCHES = {"moe_topk_f32": 1, "moe_router_topk": 1, "moe_router_topk_placed": 1,
              "moe_router_gemm_topk": 1,
              "moe_row_id_map": 3,

@@ -250,6 +250,21 @@ def test_gemm_few_rows(cuda_dev, splits, n, k, layout):
         _check_swiglu(q, pre, y, s, k)
 
 
+@pytest.mark.parametrize("splits", [[3, 1597], [0, 1, 128, 1919], [129, 2, 0, 1300, 17], [40, 200, 5], [255, 1, 256, 128]])
+@pytest.mark.parametrize("layout", ["NK", "KN"])
+def test_gemm_small_groups_beside_large(cuda_dev, splits, layout):
+    """Calls of one launch (512 rows a group and more) and of two, each followed by a reader of all rows."""
+    import moe_b200
+    rows, k = sum(splits), 1040
+    x, w = _operands(cuda_dev, rows, len(splits), 528, k, layout, 23)
+    plan = moe_b200.GroupedGemmPlan(len(splits), cuda_dev).from_splits(torch.tensor(splits))
+    want, s = _product64(x, w, splits, layout)
+    for _ in range(20):
+        again = moe_b200.grouped_gemm_fp8(x, w, plan=plan, w_layout=layout).double()  # reads behind the launches
+        assert bool(((again - want).abs() <= 2.0 ** -8 * want.abs() + 1.01 * k * 2.0 ** -24 * s).all())
+    assert plan.device_error() == 0
+
+
 def test_gemm_rows_of_no_group_stay(cuda_dev):
     """Rows behind the last group, also inside its last tile, are not written."""
     import moe_b200
