@@ -11,17 +11,18 @@
 // (16384 tokens x 256 experts always hold such pairs), so it is that of c and
 // group values formed and compared in 64 bits. A first pass in fp32 with an
 // error bound settles the rows where no decision is that close; the others
-// (one in some hundred) are selected in 64 bits.
+// (one in some hundred) are ordered or selected in 64 bits.
 //
 // One warp per token: a row is a kilobyte, its group maxima and its selection
 // are exchanges between lanes, and nothing has to leave the warp. A lane
 // holds consecutive columns of one group, so that a group is a few lanes.
 // Bound by instruction issue, and at the end by the latency of a row that
-// needs 64 bits (without them 3 us less; selected by a copy of c in shared
-// memory they took 10 us of 34): 16384 x 256, 8 groups of which 4 stay, top-8:
-// 24.5 us on the device against 6.0 us of bytes (28.5 with __expf and
-// __fdividef, which cover subnormal numbers, and with checks of every column);
-// 8192 x 1024, one group: 48 us; 4 tokens: 4.8 us.
+// needs 64 bits (16384 x 256, 8 groups of which 4 stay, top-8: selected by a
+// copy of c in shared memory 10 us of 34, in registers 3 of 24; rows where the
+// order of the taken experts alone is open, most of them, evaluate only
+// those): 22.7 us on the device against 6.0 us of bytes (4 us more with __expf
+// and __fdividef, which cover subnormal numbers, and with checks of every
+// column); 8192 x 1024, one group: 50 us; 4 tokens: 4.8 us.
 // The gradient reads what a row needs and writes it once: 16384 x 256 from a
 // sigmoid 7.7 us (2.9 us of bytes; 9.8 with a warp a token).
 #include <math.h>
@@ -193,12 +194,13 @@ struct RouteArgs {
 // Fast selection in fp32 with an error bound. Each lane holds vpl consecutive
 // columns of one group, `lanes` lanes a group. c in fp32 is off by at most
 // `err` (below), so an order of fp32 values is the true one where neighbours
-// differ by more than 2 err. Returns false, in every lane, where a decision
-// hangs on less than that (0.5 % of the rows of normal logits), or at a NaN;
-// the caller then selects in 64 bits. kFull: every lane holds VPL columns, a
+// differ by more than 2 err. Says, in every lane, what is open where a decision
+// hangs on less than that (0.5 % of the rows of normal logits): kOpen which
+// experts are taken, or a NaN is there; kOrder only in which order. kFull: every lane holds VPL columns, a
 // multiple of 4, and the rows are 16-byte aligned.
+enum Settled { kOpen, kOrder, kAll };
 template <int VPL, bool kFull>
-MOE_DEVICE bool select32(const RouteArgs& a, const float* x, int* s_mine, int& mine) {
+MOE_DEVICE Settled select32(const RouteArgs& a, const float* x, int* s_mine, int& mine) {
   const int lane = lane_id();
   const int size = a.E / a.groups;
   const int g = lane / a.lanes;
@@ -341,11 +343,29 @@ MOE_DEVICE bool select32(const RouteArgs& a, const float* x, int* s_mine, int& m
   mine = lane < a.k ? s_mine[lane] : 0;
   odd |= __reduce_add_sync(0xffffffffu, wins) != static_cast<uint32_t>(a.k);
   // Rounds whose keys lie too close (equal ones of one lane come up in
-  // consecutive rounds) leave their order open; so does an empty round.
+  // consecutive rounds) leave their order open, the last of them against the
+  // border also the choice; so does an empty round.
   const uint32_t before = __shfl_up_sync(0xffffffffu, won, 1);
-  if (lane < a.k) odd |= won == 0u;
-  if (lane >= 1 && lane <= a.k && won != 0u) odd |= !(key32_value(before) - key32_value(won) > gap);
-  return !__any_sync(0xffffffffu, odd);
+  const bool close =
+      lane >= 1 && lane <= a.k && won != 0u && !(key32_value(before) - key32_value(won) > gap);
+  odd |= (lane < a.k && won == 0u) || (lane == a.k && close);
+  if (__any_sync(0xffffffffu, odd)) return kOpen;
+  return __any_sync(0xffffffffu, close) ? kOrder : kAll;
+}
+
+// The taken experts in the order of their 64-bit scores.
+MOE_DEVICE int order64(const Scores64& sc, int k, int mine, int* s_mine) {
+  const int lane = lane_id();
+  const uint64_t key = lane < k ? order_key(sc.c(mine)) : 0;
+  int rank = 0;
+  for (int j = 0; j < k; ++j) {
+    const uint64_t other = __shfl_sync(0xffffffffu, key, j);
+    const int e = __shfl_sync(0xffffffffu, mine, j);
+    rank += other > key || (other == key && e < mine);
+  }
+  if (lane < k) s_mine[rank] = mine;
+  __syncwarp();
+  return lane < k ? s_mine[lane] : 0;
 }
 
 // The larger of two 64-bit keys over the warp, as two 32-bit maxima; `owners`
@@ -450,9 +470,9 @@ __global__ void __launch_bounds__(32 * kWarps) router_group_kernel(const RouteAr
       for (int e = lane; e < a.E; e += 32) row[e] = 0;
   }
   int mine = 0;
-  bool done = false;
+  Settled settled = kOpen;
   __shared__ int s_mine[kWarps][kMaxK];
-  if constexpr (VPL > 0) done = select32<VPL, kFull>(a, x, s_mine[warp_id()], mine);
+  if constexpr (VPL > 0) settled = select32<VPL, kFull>(a, x, s_mine[warp_id()], mine);
   Scores64 sc{x, a.bias, 0.0, 1.0, a.softmax != 0, false};
   // The softmax's normaliser cancels in renormalised weights, so that only
   // the 64-bit selection and plain softmax weights need it.
@@ -461,9 +481,10 @@ __global__ void __launch_bounds__(32 * kWarps) router_group_kernel(const RouteAr
     for (int e = lane; e < a.E; e += 32) m = fmaxf(m, __ldg(x + e));
     sc.m = warp_maxf(m);
     sc.none = sc.m == -INFINITY;
-    if (!done || !a.renorm) sc.z = softmax_sum64(x, a.E, sc.m);
+    if (settled != kAll || !a.renorm) sc.z = softmax_sum64(x, a.E, sc.m);
   }
-  if (!done) {
+  if (settled == kOrder) mine = order64(sc, a.k, mine, s_mine[warp_id()]);
+  if (settled == kOpen) {
     if constexpr (VPL > 0)
       mine = select64_lanes<VPL>(a, sc, s_mine[warp_id()]);
     else
