@@ -191,14 +191,16 @@ struct RouteArgs {
   float* probs;
 };
 
+enum Settled { kOpen, kOrder, kAll };
+
 // Fast selection in fp32 with an error bound. Each lane holds vpl consecutive
 // columns of one group, `lanes` lanes a group. c in fp32 is off by at most
 // `err` (below), so an order of fp32 values is the true one where neighbours
-// differ by more than 2 err. Says, in every lane, what is open where a decision
-// hangs on less than that (0.5 % of the rows of normal logits): kOpen which
-// experts are taken, or a NaN is there; kOrder only in which order. kFull: every lane holds VPL columns, a
-// multiple of 4, and the rows are 16-byte aligned.
-enum Settled { kOpen, kOrder, kAll };
+// differ by more than 2 err. Where a decision hangs on less than that (0.5 % of
+// the rows of normal logits) every lane gets what is open: kOpen, which experts
+// are taken (or a NaN is there); kOrder, only their order.
+// kFull: every lane holds VPL columns, a multiple of 4, and the rows are
+// 16-byte aligned.
 template <int VPL, bool kFull>
 MOE_DEVICE Settled select32(const RouteArgs& a, const float* x, int* s_mine, int& mine) {
   const int lane = lane_id();
