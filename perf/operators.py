@@ -14,7 +14,6 @@ Four operators, each with its directions:
 8-bit tensors are returned in their own types (float8_e4m3fn values and float8_e8m0fnu scales), whose elements stand
 for numbers. With `own` false run() is the plain form in elementary torch operations, with `own` true the framework's.
 """
-import functools
 import math
 import sys
 from pathlib import Path
@@ -28,7 +27,6 @@ BLK = 128
 FMAX = 448.0  # largest e4m3 value
 
 
-@functools.lru_cache(None)
 def _pkg():
     """This repository's package (its folder is not a Python identifier, so it is put on the path)."""
     root = str(Path(__file__).resolve().parent.parent / "1188b-reference-kernels_b200")
