@@ -305,7 +305,8 @@ MOE_DEVICE Settled select32(const RouteArgs& a, const float* x, int* s_mine, int
 #pragma unroll
   for (int j = 0; j < VPL; ++j) key[j] = in && (kFull || j < n) && !odd ? order_key32(c[j]) : 0u;
   // A lane offers its best column; its second best stands ready, and only a
-  // lane that wins a third time looks through its columns again.
+  // lane that wins a second time looks through its columns again. It passes
+  // over those it has given, not over their keys: others may have equal ones.
   uint32_t b1 = 0, b2 = 0;
   int c1 = 0, c2 = 0;
 #pragma unroll
@@ -318,6 +319,7 @@ MOE_DEVICE Settled select32(const RouteArgs& a, const float* x, int* s_mine, int
   }
   bool spare = true;
   uint32_t wins = 0;
+  uint32_t given = 0;               // bit j: column j has been taken
   uint32_t won = 0;                 // lane r: the key of round r
   for (int r = 0; r <= a.k; ++r) {  // one more than is taken: the border below
     const uint32_t w = __reduce_max_sync(0xffffffffu, b1);
@@ -326,6 +328,7 @@ MOE_DEVICE Settled select32(const RouteArgs& a, const float* x, int* s_mine, int
     if (b1 == w) {  // one lane, or several of equal keys: the wins then add up to more than k
       ++wins;
       s_mine[r] = col0 + c1;
+      given |= 1u << c1;
       if (spare) {
         b1 = b2;
         c1 = c2;
@@ -334,7 +337,7 @@ MOE_DEVICE Settled select32(const RouteArgs& a, const float* x, int* s_mine, int
         b1 = 0;
 #pragma unroll
         for (int j = 0; j < VPL; ++j) {
-          const bool next = key[j] < w && key[j] > b1;
+          const bool next = !(given >> j & 1u) && key[j] > b1;
           b1 = next ? key[j] : b1;
           c1 = next ? j : c1;
         }
@@ -344,8 +347,8 @@ MOE_DEVICE Settled select32(const RouteArgs& a, const float* x, int* s_mine, int
   __syncwarp();
   mine = lane < a.k ? s_mine[lane] : 0;
   odd |= __reduce_add_sync(0xffffffffu, wins) != static_cast<uint32_t>(a.k);
-  // Rounds whose keys lie too close (equal ones of one lane come up in
-  // consecutive rounds) leave their order open, the last of them against the
+  // Rounds whose keys lie too close (equal ones of one lane come up one round
+  // after the other) leave their order open, the last of them against the
   // border also the choice; so does an empty round.
   const uint32_t before = __shfl_up_sync(0xffffffffu, won, 1);
   const bool close =
