@@ -527,14 +527,24 @@ void launch_route(const RouteArgs& a, cudaStream_t s) {
 }
 
 // kLanes lanes per token, of which lane j < k holds the j-th selected expert.
-//   renorm: ds_j = scale * (g_j / S - (sum_i g_i s_i) / S^2), S = sum_i s_i;  else ds_j = scale * g_j
-//   sigmoid: dx_j = ds_j s_j (1 - s_j), 0 elsewhere; logits: dx_j = ds_j
-//   softmax: dx_e = s_e (ds_e - sum_j ds_j s_j), ds 0 outside the selection
-// With renorm the softmax's normaliser cancels: the weights are a softmax w of
-// the selected logits alone, dx_j = w_j (g_j - sum_i g_i w_i), exactly 0
-// elsewhere, and the rest of the row is not read.
+// With renorm the weights are w_j = s_j / S, S = sum_i s_i, and
+//   sigmoid: dx_j = scale * w_j (1 - s_j) (g_j - sum_i g_i w_i)
+//   softmax: dx_j = scale * w_j (g_j - sum_i g_i w_i): its normaliser cancels, w is a softmax of the selected
+//            logits alone and the rest of the row is not read
+//   logits:  dx_j = scale * (g_j - sum_i g_i w_i) / S
+// and 0 elsewhere; nothing is divided by S twice, whose square leaves fp32's
+// range long before the weights do. Without:
+//   sigmoid: dx_j = scale * g_j s_j (1 - s_j)     logits: dx_j = scale * g_j
+//   softmax: dx_e = s_e (ds_e - sum_j ds_j s_j), ds_j = scale * g_j, 0 outside the selection
+// Of a sigmoid, q = e^-|x| gives s and 1 - s as 1 / (1 + q) and q / (1 + q),
+// neither by a difference. Its w_j come from numerators e^min(x,0) relative to
+// the list's largest, so that a list of tiny scores keeps its weights.
 // What a token waits for is its list, then the gathers; with as few lanes a
 // token as its list needs, a warp has those of several under way.
+// 64-bit sigmoid scores of logits at or below this are 0, and so are the
+// forward's weights of a list that holds no other.
+constexpr float kNoScore = -709.7827f;
+
 template <int kLanes>
 MOE_DEVICE float group_sum(float v) {
 #pragma unroll
@@ -575,39 +585,52 @@ __global__ void __launch_bounds__(32 * kWarps) router_backward_kernel(
         sum += expf(__ldg(x + e) + (bias ? __ldg(bias + e) : 0.f) - m);
     z = warp_sumf(sum);
   }
-  auto score = [&](int e) {
-    const float v = __ldg(x + e) + (bias ? __ldg(bias + e) : 0.f);
-    if (mode == 2) return 1.0f / (1.0f + expf(-v));
-    if (row_softmax) return m > -INFINITY ? expf(v - m) / z : 0.f;
-    return v;  // list_softmax: the exponential follows once the list's maximum is known
-  };
+  auto logit = [&](int e) { return __ldg(x + e) + (bias ? __ldg(bias + e) : 0.f); };
+  auto row_score = [&](int e) { return m > -INFINITY ? expf(logit(e) - m) / z : 0.f; };
   int col = -1;  // this lane's expert, as a column of the logits
-  float s = 0.f, g = 0.f;
+  float v = 0.f, g = 0.f;
   if (l < k && t < T) {
     const int64_t slot = __ldg(idx + t * k + l);
     if (slot >= 0 && slot < E) col = perm ? __ldg(perm + slot) : static_cast<int>(slot);
     if (col >= 0 && col < E) {
       g = scale * (grad_vals ? __ldg(grad_vals + t * k + l) : __ldg(grad_probs + t * E + slot));
-      s = score(col);
+      v = logit(col);
     } else {
       col = -1;  // named by neither the list nor the placement: no gradient
     }
   }
-  if (list_softmax) {
-    m = group_max<kLanes>(col >= 0 ? s : -INFINITY);
-    s = col >= 0 && m > -INFINITY ? expf(s - m) : 0.f;
-    const float S = group_sum<kLanes>(s);
-    s = S == 0.f ? 0.f : s / S;
-  }
-  float ds = g;
-  if (list_softmax) {
-    ds = g - group_sum<kLanes>(g * s);
+  // dx_j = ds * factor
+  float ds = g, factor = 1.f;
+  float dot = 0.f;  // of a softmax over the row
+  if (mode == 2) {
+    const float q = expf(-fabsf(v));
+    const float r = 1.0f / (1.0f + q);
+    const bool up = v >= 0.f;
+    factor = up ? q * r : r;  // 1 - s
+    if (renorm) {
+      const float top = fminf(v, 0.f);
+      m = group_max<kLanes>(col >= 0 ? top : -INFINITY);
+      float w = col >= 0 && m > kNoScore ? expf(top - m) * r : 0.f;
+      const float S = group_sum<kLanes>(w);
+      w = S == 0.f ? 0.f : w / S;
+      ds = w * (g - group_sum<kLanes>(g * w));
+    } else {
+      ds = g * (up ? r : q * r);
+    }
+  } else if (list_softmax) {
+    m = group_max<kLanes>(col >= 0 ? v : -INFINITY);
+    float w = col >= 0 && m > -INFINITY ? expf(v - m) : 0.f;
+    const float S = group_sum<kLanes>(w);
+    w = S == 0.f ? 0.f : w / S;
+    ds = w * (g - group_sum<kLanes>(g * w));
+  } else if (row_softmax) {
+    factor = col >= 0 ? row_score(col) : 0.f;
+    dot = warp_sumf(ds * factor);
   } else if (renorm) {
-    const float S = group_sum<kLanes>(s);
-    const float dot = group_sum<kLanes>(g * s);
-    ds = S == 0.f ? 0.f : g / S - dot / (S * S);
+    const float S = group_sum<kLanes>(v);
+    const float mean = group_sum<kLanes>(S == 0.f ? 0.f : g * (v / S));
+    ds = S == 0.f ? 0.f : (g - mean) / S;
   }
-  const float dot = row_softmax ? warp_sumf(ds * s) : 0.f;
   // an expert named twice gets the sum of its gradients
   float dsum = 0.f;
   for (int j = 0; j < k; ++j) {
@@ -616,7 +639,7 @@ __global__ void __launch_bounds__(32 * kWarps) router_backward_kernel(
     if (cj == col) dsum += dj;
   }
   if (row_softmax) {
-    for (int e = lane; e < E; e += 32) o[e] = -score(e) * dot;
+    for (int e = lane; e < E; e += 32) o[e] = -row_score(e) * dot;
   } else {  // the warp's rows lie one behind the other
     float* first = out + t0 * E;
     const int64_t values = (T - t0 < kTokens ? T - t0 : kTokens) * E;
@@ -627,13 +650,7 @@ __global__ void __launch_bounds__(32 * kWarps) router_backward_kernel(
       for (int64_t e = lane; e < values; e += 32) first[e] = 0.f;
   }
   __syncwarp();
-  if (col >= 0) {
-    float d = dsum;
-    if (mode == 2) d = dsum * s * (1.0f - s);
-    if (row_softmax) d = s * (dsum - dot);
-    if (list_softmax) d = s * dsum;
-    o[col] = d;
-  }
+  if (col >= 0) o[col] = (dsum - dot) * factor;
 }
 
 template <int kLanes, typename... Args>
