@@ -10,8 +10,11 @@
 // The selection hangs on the last bits of c wherever two experts come close
 // (16384 tokens x 256 experts always hold such pairs), so it is that of c and
 // group values formed and compared in 64 bits. A first pass in fp32 with an
-// error bound settles the rows where no decision is that close; the others
-// (one in some hundred) are ordered or selected in 64 bits.
+// error bound settles the rows where no decision is that close; the others are
+// ordered or selected in 64 bits. Of 16384 rows of 256 normal logits, top-8,
+// that is 0.05 % with sigmoid and 0.2 % with softmax scores, mostly only to be
+// ordered; of the same logits rounded to bf16, where equal scores are common,
+// 39 % (20 us more for one group).
 //
 // One warp per token: a row is a kilobyte, its group maxima and its selection
 // are exchanges between lanes, and nothing has to leave the warp. A lane
@@ -196,9 +199,9 @@ enum Settled { kOpen, kOrder, kAll };
 // Fast selection in fp32 with an error bound. Each lane holds vpl consecutive
 // columns of one group, `lanes` lanes a group. c in fp32 is off by at most
 // `err` (below), so an order of fp32 values is the true one where neighbours
-// differ by more than 2 err. Where a decision hangs on less than that (0.5 % of
-// the rows of normal logits) every lane gets what is open: kOpen, which experts
-// are taken (or a NaN is there); kOrder, only their order.
+// differ by more than 2 err. Where a decision hangs on less than that, every lane
+// gets what is open: kOpen, which experts are taken (or a NaN is there); kOrder,
+// only their order.
 // kFull: every lane holds VPL columns, a multiple of 4, and the rows are
 // 16-byte aligned.
 template <int VPL, bool kFull>
@@ -228,13 +231,18 @@ MOE_DEVICE Settled select32(const RouteArgs& a, const float* x, int* s_mine, int
   load(x, -INFINITY, v);
   if (a.bias != nullptr) load(a.bias, 0.f, add);
   // fp32 scores and what they may be off by, in units of 2^-23.
-  // fast_exp(t) is off by 2 + 1.18 |t| of itself, fast_rcp by 1, its use by 1.
+  // fast_exp(t) is off by 2 + 1.18 |t| of itself (the CUDA C++ Programming
+  // Guide's bound of __expf, these two steps: 2 + 1.173 |t| ulp), fast_rcp by 1
+  // (PTX ISA, rcp.approx), its use by 1.
   // sigmoid: of exp's error s (1 - s) arrives, at most 1/4 * 2 + 1.18 * 0.23;
   //   the sum 1 + e adds 1/2, the quotient 2: together below 4.
-  // softmax: t = x - m adds |t| / 2 to exp's; s |t| <= 1/e (z >= 1), so
-  //   s (2 + 1.68 |t|) <= 2 s + 0.62; z inherits the mean of 2 + 1.68 |t|
-  //   under s (at most 2 + 1.68 ln 512) and (16 + 5) / 2 for its own sums;
-  //   quotient and product add 2.5: together below 1 + 30 s, s <= 1 / z.
+  // softmax: t = x - m adds |t| / 2 to exp's; s |t| <= rz / e, so that
+  //   s (2 + 1.68 |t|) <= 2.62 rz. z inherits the mean of 2 + 1.68 |t| under s;
+  //   that of |t| is s's entropy less ln z, at most ln E, E <= 32 VPL. Its own
+  //   sums, VPL terms in a row and five steps between lanes, add (VPL + 5) / 2,
+  //   quotient and product 2.5. With s <= rz the total is
+  //   (9.7 + 1.68 ln(32 VPL) + VPL / 2) rz: 37.3 for 32 columns (23.0 for 8),
+  //   in the code 1 + (22 + VPL / 2) rz, 38 (26).
   // Adding the bias rounds once more, 2^-24 |c|.
   float m = 0.f, rz = 1.f, err;
   if (a.softmax) {
@@ -246,7 +254,7 @@ MOE_DEVICE Settled select32(const RouteArgs& a, const float* x, int* s_mine, int
 #pragma unroll
     for (int j = 0; j < VPL; ++j) z += kFull || j < n ? fast_exp(v[j] - m) : 0.f;
     rz = fast_rcp(warp_sumf(z));
-    err = (1.f + 30.f * rz) * 1.1920929e-7f;
+    err = (1.f + (22 + VPL / 2) * rz) * 1.1920929e-7f;
   } else {
     err = 4.f * 1.1920929e-7f;
   }
@@ -450,8 +458,9 @@ MOE_DEVICE int select64_lanes(const RouteArgs& a, const Scores64& sc, int* s_min
 }
 
 // One warp per token. VPL 0: 64 bits throughout, the scores in shared memory
-// (shapes whose lanes would hold more than 32 columns: 17 to 31 groups that
-// leave lanes without any).
+// (shapes whose lanes would hold more than 32 columns, where a number of groups
+// that is no power of two leaves lanes without any: 3 groups of 341, 9 of 113,
+// 17 of 60).
 template <int VPL, bool kFull>
 __global__ void __launch_bounds__(32 * kWarps) router_group_kernel(const RouteArgs a) {
   extern __shared__ double s_c[];
