@@ -804,21 +804,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!ok && lane == 0) raise_abort(abort_flag, p.err, kErrEpilogue);
   }
 
-  tc_fence_before();
-  __syncthreads();
-  if constexpr (kPair) cluster_sync();  // no CTA leaves while its partner may still touch its memory
-  if (warp == 1) {
-    tc_fence_after();
-    if constexpr (kPair)
-      tmem_dealloc_pair(tmem, kTmemCols);
-    else
+  if constexpr (kPair) {
+    pair_teardown(tmem, kTmemCols, warp == 1);
+  } else {
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+      tc_fence_after();
       tmem_dealloc(tmem, kTmemCols);
+    }
+    // What follows in the stream waits for this launch alone, so it ends after the pairs'.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
   }
-  // What follows in the stream waits for this launch alone, so it ends after the pairs'.
-  if constexpr (!kPair) asm volatile("griddepcontrol.wait;" ::: "memory");
-  // Neither SM is given to another kernel's CTA, which allocates TMEM, before
-  // both have released the pair's.
-  if constexpr (kPair) cluster_sync();
 }
 
 // 3-D tensor map over bytes [d2, d1, d0] (d0 contiguous), box 128 x box_rows x 1,

@@ -619,13 +619,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!ok && lane == 0) raise_abort(abort_flag, p.err, kErrTimeoutEpilogue);
   }
 
-  tc_fence_before();
-  __syncthreads();
-  cluster_sync();  // no CTA leaves while its partner may still touch its memory
-  if (warp == 1) {
-    tc_fence_after();
-    tmem_dealloc_pair(tmem_base, kTmemCols);
-  }
+  pair_teardown(tmem_base, kTmemCols, warp == 1);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {

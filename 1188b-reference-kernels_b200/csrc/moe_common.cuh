@@ -377,6 +377,22 @@ MOE_DEVICE void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
   asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols)
                : "memory");
 }
+// End of a pair kernel, for all threads of both CTAs. No CTA goes on while its
+// partner may still touch its memory; `owner` (one warp of each CTA) releases
+// the pair's TMEM; and neither SM is given to another kernel's CTA, which may
+// allocate TMEM of its own there, before both warps have released. With one
+// stream the next kernel waits for both CTAs anyway; kernels of other streams
+// do not.
+MOE_DEVICE void pair_teardown(uint32_t tmem, uint32_t ncols, bool owner) {
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  if (owner) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, ncols);
+  }
+  cluster_sync();
+}
 // D[tmem of both CTAs] (+)= A * B^T over the CTA pair (M = 256 split by rows,
 // B split by N halves), issued by one thread of the leader CTA.
 MOE_DEVICE void umma_bf16_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,

@@ -588,13 +588,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!ok && lane == 0) raise_abort(abort_flag, p.err, kErrTimeoutEpilogue);
   }
 
-  tc_fence_before();
-  __syncthreads();
-  cluster_sync();  // no CTA leaves while its partner may still touch its memory
-  if (warp == 1) {
-    tc_fence_after();
-    tmem_dealloc_pair(tmem_base, p.tmem_cols);
-  }
+  pair_teardown(tmem_base, p.tmem_cols, warp == 1);
 }
 
 size_t smem_bytes(int stages, int E, int k) {

@@ -98,9 +98,10 @@ class MoELayer:
     """Forward of one MoE expert layer on one GPU (inputs already on device).
 
     A layer keeps one group table: run it on one stream at a time. Backward
-    passes of different layers are for one stream at a time as well (two at
-    once, one of them a replayed graph, once met an illegal access whose cause
-    is not known)."""
+    passes of different layers are for one stream at a time as well: two at
+    once, one of them a replayed graph, once met an illegal access. The one
+    window found, between the two CTAs of a pair that release their TMEM, is
+    closed, but that it was the cause is not shown."""
 
     def __init__(self, weights: Union[MoEWeights, MoEWeightsFp8], topk: int = 8,
                  renorm: bool = True, expert_bias: Optional[torch.Tensor] = None,
