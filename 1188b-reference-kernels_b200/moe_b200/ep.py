@@ -34,7 +34,7 @@ import torch.distributed as dist
 from . import _lib
 
 from . import ops
-from .layer import MoEWeights
+from .layer import MoEWeights, MoEWeightsFp8
 
 
 class EPDispatcher:
@@ -502,9 +502,8 @@ class MoELayerEP:
         no data and never wait on each other on the device. The output is the
         same, bit for bit, as with C = 1 (same receive rows, same GEMM
         groups, same combine)."""
-        if not isinstance(local_weights, MoEWeights):
-            raise ValueError("MoELayerEP exchanges bf16 rows: it takes MoEWeights, not "
-                             f"{type(local_weights).__name__}")
+        if isinstance(local_weights, MoEWeightsFp8):
+            raise ValueError("MoELayerEP exchanges bf16 rows: it takes MoEWeights, not MoEWeightsFp8")
         self.placement = placement
         self.disp = EPDispatcher(num_experts, group)
         self.peer = None
