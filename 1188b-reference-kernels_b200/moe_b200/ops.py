@@ -453,7 +453,7 @@ class GroupedGemmPlan:
         self.nbytes = nb.value
         self.workspace = _workspace(self.nbytes, device)
         self.workspace[:256].zero_()  # error word reads 0 before the first plan
-        self.device = device
+        self.device = self.workspace.device  # with its index, whatever form `device` has
         self.num_w = 0  # weight matrices that the table names, once it is built
 
     def from_splits(self, m_splits: torch.Tensor, align: int = 1) -> "GroupedGemmPlan":
