@@ -5,7 +5,8 @@
 //             once and stored k times
 //   weight    w [G,N,K] -> data [G,N,K], scale [G,ceil(N/128),ceil(K/128)]: one scale for 128 x 128 values, so
 //             the same tensor serves the product with w and, read the other way, with its transpose
-//   read      data, scale -> bf16 rows (exact: an e4m3 number times a power of two)
+//   read      data, scale -> bf16 rows: an e4m3 number times a power of two, exact within bf16's range (below
+//             2^-133 results are rounded, from 2^128 on they are infinite)
 //
 // All four only move bytes; K is a multiple of 16, so that a thread holds 16
 // values (one 16-byte store) and eight lanes a block. The values stay packed

@@ -106,7 +106,10 @@ def quantize_fp8_weight(w: torch.Tensor) -> Fp8Tensor:
 
 
 def dequantize_fp8(q: Fp8Tensor) -> torch.Tensor:
-    """bf16 rows of a quantised [M,K] tensor (exact: e4m3 times a power of two)."""
+    """bf16 rows of a quantised [M,K] tensor: e4m3 times a power of two, exact
+    within bf16's range. Results below 2^-133 are rounded (under the smallest
+    scales of fp32 rows alone); values from 1.9375 * 2^127 on were rounded to
+    2^128, which reads back as infinity."""
     dev = _same_device(data=q.data, scale=q.scale)
     if q.data.dim() != 2:
         raise ValueError(f"q.data must be [M,K], got {tuple(q.data.shape)}")

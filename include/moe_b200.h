@@ -351,7 +351,9 @@ int moe_quantize_fp8(const void* x, int32_t src_type, int64_t M, int64_t K, void
 /* block of 128 x 128, [G,ceil(N/128),ceil(K/128)]. G <= 65535.               */
 int moe_quantize_fp8_weight(const void* w, int32_t src_type, int64_t G, int64_t N, int64_t K,
                             void* data, void* scale, moe_stream_t stream);
-/* moe_dequantize_fp8: data [M,K], scale -> out [M,K] bf16 (exact).           */
+/* moe_dequantize_fp8: data [M,K], scale -> out [M,K] bf16, exact within      */
+/* bf16's range: results below 2^-133 are rounded; from 2^128 on, which       */
+/* values of 1.9375 * 2^127 and more round to, they are infinite.             */
 int moe_dequantize_fp8(const void* data, const void* scale, int64_t M, int64_t K, void* out,
                        moe_stream_t stream);
 /* moe_permute_fp8: quantises the rows of x [T,H] bf16 and writes row t to    */
