@@ -33,8 +33,9 @@
 // the rest of a tile's epilogue overlaps the next tile's mainloop.
 // Measured (one B200 at its 1000 W, 1.2 to 1.5 GHz): 32 groups of 1024 rows,
 // K 7168, N 4096 with SwiGLU 0.88-0.92 ms, K 2048, N 7168 0.48-0.51 ms (2150
-// and 1950 TFLOP/s; power bounds both); 20 groups of one or two rows 111-120 us,
-// 4.9-5.3 TB/s of weights.
+// and 1950 TFLOP/s, at the power limit with the tensor pipe busy 68 to 72 %: it
+// stands still at the hand-over between tiles and for the scale copies); 20
+// groups of one or two rows 103-129 us by box, 4.6-5.7 TB/s of weights.
 // Rows are described by the group table of moe_grouped_gemm_plan_*. Every
 // wait is bounded (2 s): on timeout the kernel records an error word, drains
 // its copies and MMAs, frees TMEM and returns.

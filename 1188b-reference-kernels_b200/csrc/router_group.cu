@@ -23,11 +23,13 @@
 // needs 64 bits (16384 x 256, 8 groups of which 4 stay, top-8: selected by a
 // copy of c in shared memory 10 us of 34, in registers 3 of 24; rows where the
 // order of the taken experts alone is open, most of them, evaluate only
-// those): 22.7 us on the device against 6.0 us of bytes (4 us more with __expf
+// those): 23.3 us on the device against 6.0 us of bytes (4 us more with __expf
 // and __fdividef, which cover subnormal numbers, and with checks of every
-// column); 8192 x 1024, one group: 50 us; 4 tokens: 4.8 us.
+// column); 8192 x 1024, one group: 44 us from a sigmoid, 49 from a softmax; 4
+// tokens: 3.9 us.
 // The gradient reads what a row needs and writes it once: 16384 x 256 from a
-// sigmoid 7.7 us (2.9 us of bytes; 9.8 with a warp a token).
+// sigmoid 9.2 us (2.9 us of bytes; a warp a token took 2 us more), from a
+// softmax without renorm, which reads its row twice, 17 to 19.
 #include <math.h>
 
 #include <type_traits>
